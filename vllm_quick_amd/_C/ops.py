@@ -21,7 +21,10 @@ from typing import Dict, Optional, Sequence, Tuple
 
 import torch
 
+from .. import _C_native
 from .._lib import check, lib
+
+_native = _C_native.ops
 
 PACK_FACTOR = 8
 
@@ -691,3 +694,64 @@ def awq_dequantize_packed(packed: PackedAWQ) -> torch.Tensor:
             lib.w4a16_dequantize_packed_f16(packed.packed_w.data_ptr(), packed.packed_sz.data_ptr(), out.data_ptr(),
                                             packed.K, packed.N, packed.G, _stream()), "awq_dequantize_packed")
     return out
+
+
+# --------------------------------------------------------------------------
+# around the products of a generating step (libserving_ops.so, include/serving_ops.h)
+# --------------------------------------------------------------------------
+def kv4_cache(num_blocks: int, block_size: int, num_kv_heads: int, head_size: int, device: torch.device) -> torch.Tensor:
+    """A zeroed paged cache of keys and values in 4 bits: uint8 [num_blocks, num_kv_heads, block_size * (head_size + 8)],
+    a scale and a least value (fp16) for each head of each token; the format is in include/serving_ops.h.  head_size is
+    64 or 128, block_size a multiple of 16 up to 4096.  A block is one piece of memory: `cache[dst] = cache[src]` copies
+    blocks."""
+    if head_size not in (64, 128):
+        raise ValueError(f"head_size must be 64 or 128, got {head_size}")
+    if block_size <= 0 or block_size % 16 or block_size > 4096:
+        raise ValueError(f"block_size must be a multiple of 16 from 16 to 4096, got {block_size}")
+    if num_blocks <= 0 or num_kv_heads <= 0:
+        raise ValueError("a cache needs blocks and heads")
+    return torch.zeros((num_blocks, num_kv_heads, block_size * (head_size + 8)), dtype=torch.uint8, device=device)
+
+
+def rope_append_kv4(positions: torch.Tensor, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
+                    cos_sin: torch.Tensor, cache: torch.Tensor, slots: torch.Tensor, interleaved: bool = False) -> torch.Tensor:
+    """One launch for what a step does between its qkv product and its attention: the rotated queries are returned, the
+    rotated keys and the values are stored in 4 bits.
+
+    query [T, heads, D], key and value [T, kv_heads, D] fp16 or bf16 (views of one qkv tensor will do), positions and
+    slots int64 [T], cos_sin fp32 [positions, rotary]: the cosines of rotary / 2 angles, then their sines; the first
+    `rotary` (a multiple of 16, 0 for none) elements of each head turn, in pairs (i, i + rotary / 2) or, `interleaved`,
+    (2 i, 2 i + 1).  slot = block * block_size + place; a slot outside the cache (a padded row's -1) stores nothing; the
+    others have to differ.  A position outside cos_sin makes NaN of what would turn."""
+    return _native.rope_append_kv4(positions, query, key, value, cos_sin, cache, slots, interleaved)
+
+
+def kv4_read(cache: torch.Tensor, slots: torch.Tensor, head_size: int,
+             dtype: torch.dtype) -> Tuple[torch.Tensor, torch.Tensor]:
+    """What slots (int64 [n]) of a 4-bit cache stand for: key and value [n, kv_heads, head_size] in fp16 or bf16, each
+    `least + code * scale` rounded once; zeros for a slot outside the cache."""
+    return _native.kv4_read(cache, slots, head_size, dtype)
+
+
+def paged_attention_kv4(query: torch.Tensor, cache: torch.Tensor, block_tables: torch.Tensor, seq_lens: torch.Tensor,
+                        scale: float, max_seq_len: int, query_start: Optional[torch.Tensor] = None, max_query_len: int = 1,
+                        window: int = 0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """softmax(scale q k^T) v over a 4-bit paged cache.
+
+    query [T, heads, D] fp16 or bf16; block_tables int32 [sequences, blocks], seq_lens int32 [sequences] (tokens in the
+    cache, the queries' own among them).  Without query_start each sequence has one query, its last token.  With
+    query_start (int32 [sequences + 1]) rows query_start[b] .. query_start[b + 1] - 1 are the last tokens of sequence b
+    and each sees what stands up to itself; window > 0: the last `window` of that.  max_seq_len and max_query_len size
+    the launch; rows past max_query_len of a sequence come back NaN.  A row that sees nothing is zero; rows of no
+    sequence are left as `out` holds them."""
+    return _native.paged_attention_kv4(query, cache, block_tables, seq_lens, scale, max_seq_len, query_start, max_query_len,
+                                       window, out)
+
+
+def token_logprobs(logits: torch.Tensor, token_ids: torch.Tensor,
+                   top_n: int = 0) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Of each row of logits [R, V] (fp16, bf16 or fp32): the log probability of token_ids[r] (int64; NaN for a token
+    outside the vocabulary) and the entropy, fp32 [R], and the top_n (0 .. 64) most likely tokens, int64 [R, top_n], the
+    lowest index first among equals, with their log probabilities, fp32 [R, top_n].  A logit of -inf is no token; a row
+    without any, or with a NaN or +inf, has NaN for all its probabilities."""
+    return _native.token_logprobs(logits, token_ids, top_n)

@@ -1,0 +1,397 @@
+// Log probabilities of given tokens, the entropy of each row and its most likely tokens, in one pass over the logits.
+//
+// A row (or, of a long one, a segment) is read once into the registers of one workgroup, which then takes from there
+// its maximum m, the sums  Z - 1 = sum exp(x - m) - 1  and  sum exp(x - m) (x - m),  and its largest elements.  Memory
+// bounds it: 2 or 4 bytes an element against about a dozen vector instructions.
+//   log p_t = x_t - m - log Z,   H = log Z - sum exp(x - m) (x - m) / Z    (both terms of H are positive: no cancellation)
+// Z - 1 is summed without the maxima themselves, so that log1p keeps its digits where one token has nearly all the
+// probability.
+// The n largest: the maxima of 64 disjoint groups of elements are ranked by one wave; the n-th of them bounds the n-th
+// largest element from below, so only elements not below it (little more than n) go to LDS, where each counts those
+// ahead of it.  Equal elements are told apart by their index, which makes the order total and the result one of its own.
+#include "kv4_cache.h"
+
+namespace {
+
+using namespace serving;
+
+constexpr int kMaxTop = 64;       // groups that are ranked for the bound
+constexpr int kCandidates = 1024;  // elements not below the bound that LDS takes; more (rows of equals) go the long way
+
+typedef unsigned long long u64;
+
+// What a segment leaves of itself for the join: its maximum, how often it occurs, the sums without it.
+struct Part {
+  float most, rest, weighted;
+  int count;
+};
+
+template <int TYPE>  // 0 fp16, 1 bf16, 2 fp32
+struct Logits {
+  static constexpr int kEach = TYPE == 2 ? 4 : 8;  // elements of 16 bytes
+  static constexpr int kBytes = TYPE == 2 ? 4 : 2;
+  static __device__ __forceinline__ float get(const u32x4& v, int i) {
+    const uint32_t w = v[TYPE == 2 ? i : i / 2];  // (a bit cast of a vector's element itself takes the first one)
+    if (TYPE == 2) return __builtin_bit_cast(float, w);
+    if (TYPE == 1) return __builtin_bit_cast(float, i & 1 ? w & 0xffff0000u : w << 16);
+    const f16x2 h = __builtin_bit_cast(f16x2, w);
+    return (float)(i & 1 ? h.y : h.x);
+  }
+  static __device__ __forceinline__ void hide(u32x4& v, int i) {  // element i becomes -inf
+    if (TYPE == 2) {
+      v[i] = 0xff800000u;
+    } else {
+      const uint32_t inf = TYPE == 1 ? 0xff80u : 0xfc00u;
+      v[i / 2] = i & 1 ? (v[i / 2] & 0xffffu) | (inf << 16) : (v[i / 2] & 0xffff0000u) | inf;
+    }
+  }
+};
+
+// A number that orders as the value does: both zeros alike, a NaN above +inf.
+__device__ __forceinline__ uint32_t ordered(float x) {
+  const uint32_t b = __builtin_bit_cast(uint32_t, x != x ? __builtin_nanf("") : x + 0.f);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float unordered(uint32_t o) {
+  return __builtin_bit_cast(float, o & 0x80000000u ? o & 0x7fffffffu : ~o);
+}
+__device__ __forceinline__ u64 key_of(float x, int index) {
+  return ((u64)ordered(x) << 32) | (uint32_t)(0xffffffffu - (uint32_t)index);
+}
+__device__ __forceinline__ int index_of(u64 key) { return (int)(0xffffffffu - (uint32_t)key); }
+
+__device__ __forceinline__ float larger(float a, float b) { return __builtin_elementwise_maximum(a, b); }  // NaN if one is
+
+template <typename V, typename F>
+__device__ __forceinline__ V wave_all(V v, F f) {
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) v = f(v, __shfl_xor(v, m));
+  return v;
+}
+
+// log Z and H from the maximum's count, the rest of Z and the weighted sum.
+__device__ __forceinline__ void finish(double count, double rest, double weighted, double& log_z, double& entropy) {
+  log_z = count == 1.0 ? log1p(rest) : log(count + rest);
+  entropy = log_z - weighted / (count + rest);
+}
+
+struct Args {
+  const uint8_t* logits;
+  long long row_stride;  // bytes
+  const int64_t* token_ids;
+  float *logprob, *entropy;
+  int64_t* top_ids;
+  float* top_logprobs;
+  Part* parts;  // [rows][segments], and behind them the keys [rows][segments][top]
+  u64* keys;
+  int vocab, top, segments, segment;
+};
+
+template <int TYPE, int THREADS, int NV>
+__global__ void __launch_bounds__(THREADS, 4) logprobs_kernel(Args a) {
+  typedef Logits<TYPE> X;
+  constexpr int kWaves = THREADS / 64;
+  constexpr float kLog2e = 1.44269504088896340736f;
+  __shared__ uint32_t lane_most[kWaves][64];
+  __shared__ float sums[kWaves][2];
+  __shared__ int counts[kWaves];
+  __shared__ u64 candidates[kCandidates];
+  __shared__ u64 wave_best[kWaves];
+  __shared__ int n_candidates;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int row = blockIdx.x / a.segments, seg = blockIdx.x - row * a.segments;
+  const int begin = seg * a.segment;                         // of this segment in its row
+  const int size = min(a.segment, a.vocab - begin);
+  const uint8_t* row_base = a.logits + row * a.row_stride;
+  const uint8_t* base = row_base + (long long)begin * X::kBytes;
+  const int skip = (int)((reinterpret_cast<uintptr_t>(base) & 15u) / X::kBytes);  // of the first 16 bytes, not ours
+  const u32x4* words = reinterpret_cast<const u32x4*>(base - skip * X::kBytes);
+  if (tid == 0) n_candidates = 0;
+
+  u32x4 v[NV];
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int e = (k * THREADS + tid) * X::kEach - skip;  // of this lane's first element in the segment
+    // (16 aligned bytes that hold one of the row's elements: never outside the pages of its tensor)
+    if (e < size && e > -X::kEach) {
+      v[k] = words[k * THREADS + tid];
+      if (e < 0 || e + X::kEach > size) {
+#pragma unroll
+        for (int i = 0; i < X::kEach; ++i)
+          if (e + i < 0 || e + i >= size) X::hide(v[k], i);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < X::kEach; ++i) X::hide(v[k], i);
+    }
+  }
+  float given = 0.f;
+  long long token = -1;
+  if (a.segments == 1 && tid == 0) {
+    token = a.token_ids[row];
+    if (token >= 0 && token < a.vocab) {
+      const uint8_t* p = row_base + token * X::kBytes;
+      given = TYPE == 2 ? *reinterpret_cast<const float*>(p)
+                        : TYPE == 1 ? __builtin_bit_cast(float, (uint32_t)*reinterpret_cast<const uint16_t*>(p) << 16)
+                                    : (float)*reinterpret_cast<const f16*>(p);
+    }
+  }
+
+  float mine = -__builtin_inff();
+#pragma unroll
+  for (int k = 0; k < NV; ++k)
+#pragma unroll
+    for (int i = 0; i < X::kEach; ++i) mine = larger(mine, X::get(v[k], i));
+  lane_most[wave][lane] = ordered(mine);
+  __syncthreads();
+  // the 64 groups: the elements of equal lanes of all waves
+  uint32_t group = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) group = max(group, lane_most[w][lane]);
+  const float most = unordered(wave_all(group, [](uint32_t p, uint32_t q) { return max(p, q); }));
+
+  float rest = 0.f, weighted = 0.f;
+  int count = 0;
+#pragma unroll
+  for (int k = 0; k < NV; ++k)
+#pragma unroll
+    for (int i = 0; i < X::kEach; ++i) {
+      const float d = fmaxf(X::get(v[k], i) - most, -10000.f);  // (-inf adds nothing, and not 0 * inf)
+      const float p = __builtin_amdgcn_exp2f(d * kLog2e);
+      rest += p;
+      weighted = __builtin_fmaf(p, d, weighted);
+    }
+  if (mine == most) {  // the few lanes that hold a maximum sum again without it
+    rest = 0.f;
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+      for (int i = 0; i < X::kEach; ++i) {
+        const float d = fmaxf(X::get(v[k], i) - most, -10000.f);
+        if (d == 0.f)
+          ++count;
+        else
+          rest += __builtin_amdgcn_exp2f(d * kLog2e);
+      }
+  }
+  rest = wave_all(rest, [](float p, float q) { return p + q; });
+  weighted = wave_all(weighted, [](float p, float q) { return p + q; });
+  count = wave_all(count, [](int p, int q) { return p + q; });
+  if (lane == 0) sums[wave][0] = rest, sums[wave][1] = weighted, counts[wave] = count;
+
+  // the n-th largest group maximum: each lane counts the groups ahead of its own
+  if (a.top > 0) {
+    int ahead = 0;
+#pragma unroll 16
+    for (int g = 0; g < 64; ++g) {
+      const uint32_t other = __builtin_amdgcn_readlane(group, g);
+      ahead += other > group || (other == group && g < lane);
+    }
+    const uint32_t bound = __builtin_amdgcn_readlane(group, __builtin_ctzll(__ballot(ahead == a.top - 1)));
+    if (ordered(mine) >= bound) {
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const int e = (k * THREADS + tid) * X::kEach - skip;
+#pragma unroll
+        for (int i = 0; i < X::kEach; ++i) {
+          const float x = X::get(v[k], i);
+          if (ordered(x) >= bound && e + i >= 0 && e + i < size) {
+            const int at = atomicAdd(&n_candidates, 1);
+            if (at < kCandidates) candidates[at] = key_of(x, begin + e + i);
+          }
+        }
+      }
+    }
+  }
+  __syncthreads();
+
+  float all_rest = 0.f, all_weighted = 0.f;
+  int all_count = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) all_rest += sums[w][0], all_weighted += sums[w][1], all_count += counts[w];
+  const bool finite = __builtin_isfinite(most);
+  const int n = n_candidates;
+  double log_z = 0.0, entropy = 0.0;
+  const long long part = (long long)row * a.segments + seg;
+  if (a.segments == 1) {
+    if (finite) finish(all_count, all_rest, all_weighted, log_z, entropy);
+    if (!finite) log_z = entropy = __builtin_nan("");
+    if (tid == 0) {
+      a.logprob[row] = token >= 0 && token < a.vocab ? (float)((double)(given - most) - log_z) : __builtin_nanf("");
+      a.entropy[row] = (float)entropy;
+    }
+  } else if (tid == 0) {
+    a.parts[part] = Part{most, all_rest, all_weighted, all_count};
+  }
+  const auto place = [&](int rank, u64 key) {
+    if (a.segments == 1) {
+      a.top_ids[(long long)row * a.top + rank] = index_of(key);
+      a.top_logprobs[(long long)row * a.top + rank] =
+          (float)((double)(unordered((uint32_t)(key >> 32)) - most) - log_z);
+    } else {
+      a.keys[part * a.top + rank] = key;
+    }
+  };
+  const int want = min(a.top, size);
+  if (a.segments > 1)
+    for (int r = want + tid; r < a.top; r += THREADS) a.keys[part * a.top + r] = 0;  // (below every element's key)
+  if (n <= kCandidates) {
+    for (int i = tid; i < n; i += THREADS) {
+      const u64 key = candidates[i];
+      int ahead = 0;
+      for (int j = 0; j < n; ++j) ahead += candidates[j] > key;
+      if (ahead < want) place(ahead, key);
+    }
+    return;
+  }
+  // Too many equals at the bound: one rank after the other over all elements.
+  u64 last = ~0ull;
+  for (int r = 0; r < want; ++r) {
+    u64 best = 0;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int e = (k * THREADS + tid) * X::kEach - skip;
+#pragma unroll
+      for (int i = 0; i < X::kEach; ++i) {
+        const u64 key = key_of(X::get(v[k], i), begin + e + i);
+        if (e + i >= 0 && e + i < size && key < last && key > best) best = key;
+      }
+    }
+    best = wave_all(best, [](u64 p, u64 q) { return p > q ? p : q; });
+    if (lane == 0) wave_best[wave] = best;
+    __syncthreads();
+    last = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) last = last > wave_best[w] ? last : wave_best[w];
+    if (tid == 0) place(r, last);
+    __syncthreads();
+  }
+}
+
+// Joins the segments of a row.
+template <int TYPE>
+__global__ void __launch_bounds__(256) join_kernel(Args a) {
+  typedef Logits<TYPE> X;
+  __shared__ double shared_log_z;
+  __shared__ float shared_most;
+  const int row = blockIdx.x, tid = threadIdx.x;
+  const Part* parts = a.parts + (long long)row * a.segments;
+  const u64* keys = a.keys + (long long)row * a.segments * a.top;
+  if (tid < 64) {
+    float most = -__builtin_inff();
+    for (int s = tid; s < a.segments; s += 64) most = larger(most, parts[s].most);
+    most = wave_all(most, [](float p, float q) { return larger(p, q); });
+    double rest = 0.0, weighted = 0.0, count = 0.0;
+    if (__builtin_isfinite(most)) {
+      for (int s = tid; s < a.segments; s += 64) {
+        const Part p = parts[s];
+        if (p.most == most) {
+          count += p.count;
+          rest += p.rest;
+          weighted += p.weighted;
+        } else if (p.most > -__builtin_inff()) {
+          const double d = (double)p.most - (double)most, f = exp(d), z = (double)p.count + p.rest;
+          rest += z * f;
+          weighted += (p.weighted + z * d) * f;
+        }
+      }
+    }
+    const auto add = [](double p, double q) { return p + q; };
+    rest = wave_all(rest, add), weighted = wave_all(weighted, add), count = wave_all(count, add);
+    double log_z = __builtin_nan(""), entropy = __builtin_nan("");
+    if (__builtin_isfinite(most)) finish(count, rest, weighted, log_z, entropy);
+    if (tid == 0) {
+      shared_log_z = log_z;
+      shared_most = most;
+      const long long token = a.token_ids[row];
+      float lp = __builtin_nanf("");
+      if (token >= 0 && token < a.vocab) {
+        const uint8_t* p = a.logits + row * a.row_stride + token * X::kBytes;
+        const float x = TYPE == 2 ? *reinterpret_cast<const float*>(p)
+                        : TYPE == 1 ? __builtin_bit_cast(float, (uint32_t)*reinterpret_cast<const uint16_t*>(p) << 16)
+                                    : (float)*reinterpret_cast<const f16*>(p);
+        lp = (float)((double)(x - most) - log_z);
+      }
+      a.logprob[row] = lp;
+      a.entropy[row] = (float)entropy;
+    }
+  }
+  __syncthreads();
+  const int n = a.segments * a.top;
+  for (int i = tid; i < n; i += 256) {
+    const u64 key = keys[i];
+    if (key == 0) continue;  // of a segment with fewer elements than ranks
+    int ahead = 0;
+    for (int j = 0; j < n; ++j) ahead += keys[j] > key;
+    if (ahead < a.top) {
+      a.top_ids[(long long)row * a.top + ahead] = index_of(key);
+      a.top_logprobs[(long long)row * a.top + ahead] =
+          (float)((double)(unordered((uint32_t)(key >> 32)) - shared_most) - shared_log_z);
+    }
+  }
+}
+
+// A workgroup of 1024 lanes holds 32 elements a lane, 7 (3) of which may belong to the row before; one of 256 a quarter.
+struct Plan {
+  int threads, segments, segment;
+};
+Plan plan(int rows, int vocab, int type) {
+  const int spare = type == 2 ? 3 : 7;
+  Plan p;
+  p.threads = vocab + spare <= 256 * 32 ? 256 : 1024;
+  const int most = p.threads * 32 - 8;
+  p.segments = vocab + spare <= p.threads * 32 ? 1 : (vocab + most - 1) / most;
+  p.segment = p.segments == 1 ? vocab : ((vocab + p.segments - 1) / p.segments + 7) / 8 * 8;
+  p.segments = (vocab + p.segment - 1) / p.segment;
+  (void)rows;
+  return p;
+}
+
+template <int TYPE>
+int launch(const Args& a, int rows, int threads, hipStream_t s) {
+  constexpr int kAll = 32 / Logits<TYPE>::kEach;
+  const dim3 grid((unsigned)rows * (unsigned)a.segments);
+  if (threads == 256)
+    hipLaunchKernelGGL((logprobs_kernel<TYPE, 256, kAll>), grid, dim3(256), 0, s, a);
+  else
+    hipLaunchKernelGGL((logprobs_kernel<TYPE, 1024, kAll>), grid, dim3(1024), 0, s, a);
+  if (a.segments > 1) {
+    const int rc = serving_after_launch();
+    if (rc != SERVING_OK) return rc;
+    hipLaunchKernelGGL((join_kernel<TYPE>), dim3((unsigned)rows), dim3(256), 0, s, a);
+  }
+  return serving_after_launch();
+}
+
+bool sizes_ok(int rows, int vocab, int top, int type) {
+  return rows > 0 && vocab > 0 && vocab <= (1 << 30) && top >= 0 && top <= kMaxTop && top <= vocab && type >= 0 && type <= 2;
+}
+
+}  // namespace
+
+extern "C" size_t serving_token_logprobs_workspace_bytes(int rows, int vocab, int top, int type) {
+  if (!sizes_ok(rows, vocab, top, type)) return 0;
+  const Plan p = plan(rows, vocab, type);
+  if (p.segments == 1) return 0;
+  return (size_t)rows * p.segments * (sizeof(Part) + (size_t)top * sizeof(u64));
+}
+
+extern "C" int serving_token_logprobs(const void* logits, long long row_stride, const int64_t* token_ids, float* logprob,
+                                      float* entropy, int64_t* top_ids, float* top_logprobs, int rows, int vocab, int top,
+                                      int type, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!logits || !token_ids || !logprob || !entropy || (top > 0 && (!top_ids || !top_logprobs))) return SERVING_E_NULL;
+  if (!sizes_ok(rows, vocab, top, type)) return SERVING_E_SHAPE;
+  const int bytes = type == 2 ? 4 : 2;
+  if (reinterpret_cast<uintptr_t>(logits) % bytes) return SERVING_E_ALIGN;
+  const Plan p = plan(rows, vocab, type);
+  if ((long long)rows * p.segments > 0x7fffffffLL) return SERVING_E_TOO_LARGE;
+  const size_t need = serving_token_logprobs_workspace_bytes(rows, vocab, top, type);
+  if (need && (!workspace || workspace_bytes < need)) return SERVING_E_WORKSPACE;
+  if (need && !aligned16(workspace)) return SERVING_E_ALIGN;
+  Args a{static_cast<const uint8_t*>(logits), row_stride * bytes, token_ids, logprob, entropy, top_ids, top_logprobs,
+         static_cast<Part*>(workspace), nullptr, vocab, top, p.segments, p.segment};
+  if (need) a.keys = reinterpret_cast<u64*>(a.parts + (size_t)rows * p.segments);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (type == 0) return launch<0>(a, rows, p.threads, s);
+  if (type == 1) return launch<1>(a, rows, p.threads, s);
+  return launch<2>(a, rows, p.threads, s);
+}

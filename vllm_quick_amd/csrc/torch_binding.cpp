@@ -36,6 +36,7 @@
 #include <tuple>
 #include <unordered_map>
 
+#include "../../include/serving_ops.h"
 #include "../../include/w4a16.h"
 
 namespace {
@@ -238,11 +239,14 @@ torch::Tensor awq_dequantize(torch::Tensor _kernel, torch::Tensor _scaling_facto
 
 }  // namespace
 
+void bind_serving_ops(pybind11::module& ops);  // serving_binding.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
-  m.doc() = "AWQ W4A16 operators on libw4a16.so (MI355X)";
+  m.doc() = "AWQ W4A16 operators on libw4a16.so, and those of libserving_ops.so (MI355X)";
   pybind11::module ops = m.def_submodule("ops", "vLLM custom operators");
   ops.def("awq_gemm", &awq_gemm, "Quantized GEMM for AWQ");
   ops.def("awq_dequantize", &awq_dequantize, "Dequantization for AWQ");
+  bind_serving_ops(ops);
   m.def("stock_kernel_calls", [] { return g_stock_calls.load(); },
         "awq_gemm calls served by the shape-agnostic stock-layout kernel since the module was loaded");
   m.def("repack_count", [] { return g_repacks.load(); }, "layers re-ordered into the private layout so far");
@@ -251,4 +255,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     g_table.clear();
   });
   m.def("abi_version", [] { return w4a16_abi_version(); });
+  m.def("serving_abi_version", [] { return serving_abi_version(); });
 }
