@@ -15,7 +15,8 @@
  *   values      [P / 16][D / 8][16][4]   the same bytes in pieces of 4 (8 elements), 16 tokens of a piece together
  *   parameters  [2][P][2] fp16           of the keys, then of the values: scale and least of each token
  * and an element stands for  least + code * scale.  A head x[D] of a token is stored as
- *   least = fp16(min x),  scale = fp16((max x - least) / 15),  code = clamp(rint((x - least) / scale), 0, 15)
+ *   least = fp16(min x),  scale = fp16((max x - least) * fp32(1 / 15)),
+ *   code = clamp(rint((x - least) / scale), 0, 15)
  * in fp32 arithmetic on the values before they are rounded to 16 bits (code = 0 where scale is 0).  A head that
  * holds a NaN or an infinity, or whose parameters fp16 cannot hold, is stored as NaN (both parameters).  The
  * parameters' type does not follow the activations': one cache serves fp16 and bf16 callers.

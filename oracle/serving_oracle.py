@@ -39,7 +39,7 @@ def rotate64(x, cos_sin, positions, interleaved):
 def quantise(x):
     """fp32 heads [..., D] -> codes (int), scale and least (fp16), by the format's definition."""
     least = x.amin(-1).half()
-    scale = ((x.amax(-1) - least.float()) / 15.0).half()
+    scale = ((x.amax(-1) - least.float()) * torch.tensor(1 / 15, dtype=torch.float32)).half()
     held = torch.isfinite(least) & torch.isfinite(scale) & torch.isfinite(x).all(-1)
     codes = torch.zeros(x.shape, dtype=torch.int64)
     on = held & (scale > 0)

@@ -17,10 +17,10 @@
 //                  4 g + 0..3 (g = lane >> 4) of both groups of 16; the format keeps the values of 16 tokens piece by
 //                  piece, so that the same 4 keys of a piece are again one 16-byte load, and one byte permutation a
 //                  word pairs the codes of neighbouring keys.
-// Roundings: queries enter exactly (scaled by a power of two into fp16's range), p_j vscale_j is rounded to fp16 once,
-// all sums are fp32.  The codes are not centred, so a rounded p_j vscale_j is off by up to 15 steps of it; what the
-// roundings take away is summed and given back times 8, the middle of the codes, which leaves the error that centred
-// codes would have (fp16 results; bf16 results are rounded coarser than what it repairs).
+// Roundings: queries enter exactly (scaled by a power of two into fp16's range), w_j = p_j vscale_j is rounded to fp16
+// once, all sums are fp32.  A code stands for zero at n_j = -least_j / vscale_j, not at 0, so w_j's rounding costs
+// (n - n_j) + n_j steps of it; the second part, w_j's error times n_j, is the same for all elements and goes into the
+// second sum (n_j to an eighth).  Only for fp16 results: bf16 ones are rounded coarser than what it repairs.
 #include "kv4_cache.h"
 
 namespace {
@@ -29,6 +29,8 @@ using namespace serving;
 
 constexpr float kNone = -1e30f;  // below every score, yet finite: differences of it are numbers
 constexpr int kTile = 32;        // keys of a step
+constexpr float kSlack = 8.f;     // a probability may stand this many powers of two above 1 before the maximum moves
+constexpr float kWeight = 0x1p7f;  // p vscale / (power of two above vscale) times this is rounded to fp16: below 2^15
 
 struct AttendArgs {
   const void* query;
@@ -47,8 +49,16 @@ struct AttendArgs {
   int window, max_query_len, splits;
 };
 
+// Uniform integers that no kernel here writes, through the scalar cache: a vector load would return behind all the
+// loads of keys that were issued before it.
+typedef const __attribute__((address_space(4))) int32_t* scalar_ints;
+__device__ __forceinline__ scalar_ints scalar(const int32_t* p) { return (scalar_ints)(uintptr_t)p; }
 __device__ __forceinline__ f16x2 as_pair(uint32_t w) { return __builtin_bit_cast(f16x2, w); }  // scale, least
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+// 1 / v to an eighth of it, from the number's bits: the line of slope -1 through (log2 v, log2 1/v) that is nearest.
+__device__ __forceinline__ float rough_reciprocal(float v) {
+  return __builtin_bit_cast(float, 0x7ef311c7u - __builtin_bit_cast(uint32_t, v));
+}
 __device__ __forceinline__ float over_groups_max(float v) {  // of the four groups of 16 lanes
   v = fmaxf(v, __shfl_xor(v, 16));
   return fmaxf(v, __shfl_xor(v, 32));
@@ -57,6 +67,9 @@ __device__ __forceinline__ float over_groups_sum(float v) {
   v += __shfl_xor(v, 16);
   return v + __shfl_xor(v, 32);
 }
+
+// Keeps a branch that is rarely taken a branch.
+__device__ __forceinline__ void stay() { asm volatile(""); }
 
 // One sequence as a wave sees it.
 struct Sequence {
@@ -68,9 +81,9 @@ struct Sequence {
 __device__ __forceinline__ Sequence sequence(const AttendArgs& a, int b) {
   Sequence s;
   const long long most = (long long)a.table_width * a.block_size;
-  s.length = max(0, (int)min((long long)a.seq_lens[b], most));
-  s.row = a.query_start ? a.query_start[b] : b;
-  s.queries = a.query_start ? a.query_start[b + 1] - s.row : 1;
+  s.length = max(0, (int)min((long long)scalar(a.seq_lens)[b], most));
+  s.row = a.query_start ? scalar(a.query_start)[b] : b;
+  s.queries = a.query_start ? scalar(a.query_start)[b + 1] - s.row : 1;
   if (s.row < 0 || s.row > a.tokens) s.row = a.tokens;
   s.queries = max(0, min(s.queries, a.tokens - s.row));
   s.before = s.length - s.queries;
@@ -81,34 +94,36 @@ template <typename T, int D, int NC>
 struct Wave {
   static constexpr int kSteps = D / 32;  // matrix instructions of 16 keys against 16 columns
   static constexpr int kRows = D / 16;   // tiles of 16 elements of the result
-  static constexpr bool kRepair = sizeof(T) == 2 && __is_same(T, f16);
-
-  struct Tile {
-    uint32_t k[2][kSteps];
-    u32x4 v[2], kp[2], vp[2];
-  };
+  static constexpr bool kRepair = __is_same(T, f16);
 
   const AttendArgs& a;
   const int c, g;
+  // the step's keys, values and parameters; each is overwritten by the next step's as soon as it is used
+  uint32_t k[2][kSteps];
+  u32x4 v[2], kp[2], vp[2];
   f16x8 q[NC][kSteps];
-  float qs[NC], al[NC];       // sum of the query, and what makes a score of a product
-  int lim[NC], low[NC];       // keys that a column sees: low .. lim - 1
-  float most[NC], sum[NC], flat[NC], lost[NC];
+  float qs[NC], al[NC];  // sum of the query, and what makes a score (in powers of two) of a product
+  int lim[NC], low[NC];  // keys that a column sees: low .. lim - 1
+  float shift[NC];       // p = 2^(al u + shift): no p passes 2^kSlack
+  float sum[NC], flat[NC];
   f32x4 o[NC][kRows];
-  float vref;                 // power of two above every vscale so far
-  const uint8_t* head_base;   // of this kv head in block 0
-  const int32_t* table;
+  float vref;                // power of two above every vscale so far
+  const uint8_t* head_base;  // of this kv head in block 0
+  scalar_ints table;
   long long block_bytes;
   int last_page;
+  const uint8_t* base[2];  // where the next step's two groups of 16 tokens are
+  int place[2];
+  bool known[2];
 
   __device__ __forceinline__ Wave(const AttendArgs& args) : a(args), c(threadIdx.x & 15), g((threadIdx.x & 63) >> 4) {}
 
   __device__ __forceinline__ void begin(const Sequence& s, int b, int kv, int col0, int cols) {
     head_base = a.cache + (long long)kv * Kv4<D>::block_bytes(a.block_size);
     block_bytes = Kv4<D>::block_bytes(a.block_size) * a.kv_heads;
-    table = a.tables + b * a.table_stride;
+    table = scalar(a.tables + b * a.table_stride);
     last_page = max(0, page_of((s.length - 1) >> 4));
-    vref = 0x1p-100f;
+    vref = 0x1p-40f;
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
       const int col = col0 + 16 * n + c;
@@ -145,8 +160,8 @@ struct Wave {
       }
       qs[n] = __builtin_ldexpf(sign * total, e - 24);
       al[n] = __builtin_ldexpf(fabsf(a.scale), 24 - e);
-      most[n] = kNone;
-      sum[n] = flat[n] = lost[n] = 0.f;
+      shift[n] = -kNone;
+      sum[n] = flat[n] = 0.f;
 #pragma unroll
       for (int m = 0; m < kRows; ++m) o[n][m] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
@@ -156,91 +171,126 @@ struct Wave {
     return a.per_block_magic ? (int)__umulhi((uint32_t)max(0, sixteenth), a.per_block_magic) : max(0, sixteenth);
   }
 
-  // The block that holds 16 tokens; their place in it.
+  // The block that holds 16 tokens (behind the last page: the last one, whose tokens there are hidden).
   __device__ __forceinline__ int block_of(int sixteenth) const { return table[min(page_of(sixteenth), last_page)]; }
 
-  __device__ __forceinline__ void load(Tile& t, int tile, int block0, int block1) const {
+  __device__ __forceinline__ void aim(int tile, int block0, int block1) {
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       const int sixteenth = 2 * tile + s, block = s ? block1 : block0;
-      const bool known = (uint32_t)block < (uint32_t)a.num_blocks;
+      known[s] = (uint32_t)block < (uint32_t)a.num_blocks;
       const int page = page_of(sixteenth);
-      // (groups of 16 behind the last page are hidden; any place in the cache serves)
-      const int place = page <= last_page ? 16 * sixteenth - page * a.block_size : 0;
-      const uint8_t* base = head_base + (known ? block : 0) * block_bytes;
-      const uint8_t* kc = base + (uint32_t)(place * Kv4<D>::kTokenBytes) + (uint32_t)(c * Kv4<D>::kTokenBytes + g * (D / 8));
+      place[s] = page <= last_page ? 16 * sixteenth - page * a.block_size : 0;
+      base[s] = head_base + (known[s] ? block : 0) * block_bytes;
+    }
+  }
+
+  __device__ __forceinline__ void load_keys() {
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const uint8_t* at = base[s] + (uint32_t)(place[s] * Kv4<D>::kTokenBytes) + (uint32_t)(c * Kv4<D>::kTokenBytes + g * (D / 8));
       if (D == 128) {
-        const u32x4 w = *reinterpret_cast<const u32x4*>(kc);
+        const u32x4 w = *reinterpret_cast<const u32x4*>(at);
 #pragma unroll
-        for (int j = 0; j < kSteps; ++j) t.k[s][j] = w[j];
+        for (int j = 0; j < kSteps; ++j) k[s][j] = w[j];
       } else {
-        const u32x2 w = *reinterpret_cast<const u32x2*>(kc);
+        const u32x2 w = *reinterpret_cast<const u32x2*>(at);
 #pragma unroll
-        for (int j = 0; j < kSteps; ++j) t.k[s][j] = w[j];
-      }
-      const int piece = D == 128 ? c : c >> 1;
-      t.v[s] = *reinterpret_cast<const u32x4*>(base + (uint32_t)(Kv4<D>::values(a.block_size) + (place / 16) * Kv4<D>::kGroupBytes) +
-                                               (uint32_t)(piece * Kv4<D>::kPieceBytes + 16 * g));
-      t.kp[s] = *reinterpret_cast<const u32x4*>(base + (uint32_t)(Kv4<D>::key_params(a.block_size) + 4 * place) + (uint32_t)(16 * g));
-      t.vp[s] = *reinterpret_cast<const u32x4*>(base + (uint32_t)(Kv4<D>::value_params(a.block_size) + 4 * place) + (uint32_t)(16 * g));
-      if (!known) {  // a block that the cache does not have: its keys are NaN
-        t.kp[s] = u32x4{0x7e007e00u, 0x7e007e00u, 0x7e007e00u, 0x7e007e00u};
+        for (int j = 0; j < kSteps; ++j) k[s][j] = w[j];
       }
     }
   }
 
-  // Scores of 32 keys to probabilities, to the B operand of the second product.
+  __device__ __forceinline__ void load_params() {
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const uint32_t at = (uint32_t)(Kv4<D>::key_params(a.block_size) + 4 * place[s]);
+      kp[s] = *reinterpret_cast<const u32x4*>(base[s] + at + (uint32_t)(16 * g));
+      vp[s] = *reinterpret_cast<const u32x4*>(base[s] + (at + 4 * (uint32_t)a.block_size) + (uint32_t)(16 * g));
+      if (!known[s])  // a block that the cache does not have: its keys are NaN
+        kp[s] = u32x4{0x7e007e00u, 0x7e007e00u, 0x7e007e00u, 0x7e007e00u};
+    }
+  }
+
+  __device__ __forceinline__ void load_values() {
+    const int piece = D == 128 ? c : c >> 1;
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+      v[s] = *reinterpret_cast<const u32x4*>(base[s] + (uint32_t)(Kv4<D>::values(a.block_size) + (place[s] / 16) * Kv4<D>::kGroupBytes) +
+                                             (uint32_t)(piece * Kv4<D>::kPieceBytes + 16 * g));
+  }
+
+  __device__ __forceinline__ bool sees(int n, int from, int i) const {
+    const int key = from + 16 * (i / 4) + 4 * g + i % 4;
+    return key >= low[n] && key < lim[n];
+  }
+
+  // Scores of 32 keys to weights, the B operand of the second product.
   template <bool MASK>
-  __device__ __forceinline__ void softmax(const Tile& t, const f32x4 (&s)[2], int n, int from, float vinv, f16x8& p) {
-    float u[8];
-    bool sees[8];
-    float top = most[n];
+  __device__ __forceinline__ void weigh(const f32x4 (&s)[2], int n, int from, float vinv, f16x8& p) {
+    float u[8], e[8], w[8], least[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const f16x2 kp = as_pair(t.kp[i / 4][i % 4]);
-      u[i] = __builtin_fmaf(s[i / 4][i % 4], (float)kp.x, (float)kp.y * qs[n]);
-      if (MASK) {
-        const int key = from + 16 * (i / 4) + 4 * g + i % 4;
-        sees[i] = key >= low[n] && key < lim[n];
-        if (!sees[i]) u[i] = kNone;
-      }
-      top = fmaxf(top, u[i]);
+      const f16x2 par = as_pair(kp[i / 4][i % 4]);
+      u[i] = __builtin_fmaf(s[i / 4][i % 4], (float)par.x, (float)par.y * qs[n]);
     }
-    top = over_groups_max(top);
-    if (__any(top > most[n])) {
-      const float f = exp2_(al[n] * (most[n] - top));
-      most[n] = top;
+    if (MASK) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) u[i] = sees(n, from, i) ? u[i] : kNone;
+    }
+    float most = u[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) most = fmaxf(most, u[i]);
+    if (__any(__builtin_fmaf(al[n], most, shift[n]) > kSlack)) {
+      stay();
+      most = over_groups_max(most);  // (a column moves for its own keys only, whatever the wave's others do)
+      const float next = __builtin_fmaf(al[n], most, shift[n]) > kSlack ? -al[n] * most : shift[n];
+      const float f = exp2_(next - shift[n]);
+      shift[n] = next;
       sum[n] *= f;
       flat[n] *= f;
-      lost[n] *= f;
 #pragma unroll
       for (int m = 0; m < kRows; ++m) o[n][m] *= f;
     }
-    const float shift = -al[n] * top;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const f16x2 vp = as_pair(t.vp[i / 4][i % 4]);
-      float e = exp2_(__builtin_fmaf(al[n], u[i], shift));
-      float w = e * ((float)vp.x * vinv), fl = e * (float)vp.y;
-      if (MASK) {  // (not 0 times what a hidden key's parameters may be)
-        e = sees[i] ? e : 0.f;
-        w = sees[i] ? w : 0.f;
-        fl = sees[i] ? fl : 0.f;
+      const f16x2 par = as_pair(vp[i / 4][i % 4]);
+      e[i] = exp2_(__builtin_fmaf(al[n], u[i], shift[n]));
+      w[i] = e[i] * ((float)par.x * vinv);
+      least[i] = (float)par.y;
+    }
+    if (MASK) {  // (not 0 times what a hidden key's parameters may be)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const bool on = sees(n, from, i);
+        e[i] = on ? e[i] : 0.f;
+        w[i] = on ? w[i] : 0.f;
+        least[i] = on ? least[i] : 0.f;
       }
-      sum[n] += e;
-      flat[n] += fl;
-      p[i] = (f16)w;
-      if (kRepair) lost[n] += w - (float)p[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      sum[n] += e[i];
+      flat[n] = __builtin_fmaf(e[i], least[i], flat[n]);
+      p[i] = (f16)w[i];
+      if (kRepair) {
+        const float vs = (float)as_pair(vp[i / 4][i % 4]).x * vinv;
+        flat[n] = __builtin_fmaf((float)p[i] - w[i], least[i] * rough_reciprocal(fmaxf(vs, 0x1p-40f)), flat[n]);
+      }
     }
   }
 
-  __device__ __forceinline__ void step(Tile& t, int from, int length, bool masked) {
+  // 32 keys.  What the running maximum and the values' scales are measured against moves only when a probability would
+  // pass 2^kSlack, or a scale its reference, which no step but the first few does: the four groups of lanes need to
+  // agree on neither until then.
+  template <bool MASK>
+  __device__ __forceinline__ void step(int from, int length) {
     f32x4 s[NC][2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
 #pragma unroll
       for (int j = 0; j < kSteps; ++j) {
-        const uint32_t w = t.k[h][j], x = w >> 8;
+        const uint32_t w = k[h][j], x = w >> 8;
         const u32x4 f = {w & 0x000f000fu, w & 0x00f000f0u, x & 0x000f000fu, x & 0x00f000f0u};
 #pragma unroll
         for (int n = 0; n < NC; ++n)
@@ -248,42 +298,38 @@ struct Wave {
                                                            j ? s[n][h] : f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
       }
     }
-    if (masked) {  // parameters behind the sequence may be anything
+    load_keys();
+    if (MASK) {  // parameters behind the sequence may be anything
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        if (from + 16 * (i / 4) + 4 * g + i % 4 >= length) t.vp[i / 4][i % 4] = 0;
+        if (from + 16 * (i / 4) + 4 * g + i % 4 >= length) vp[i / 4][i % 4] = 0;
     }
-    float ref = 0.f;
+    f16x2 big = as_pair(vp[0][0]);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) ref = fmaxf(ref, (float)as_pair(t.vp[i / 4][i % 4]).x);
-    ref = over_groups_max(ref);
-    if (__any(ref >= vref)) {
-      const float next = __builtin_ldexpf(1.f, __builtin_amdgcn_frexp_expf(ref)), f = vref / next;
+    for (int i = 1; i < 8; ++i) big = __builtin_elementwise_max(big, as_pair(vp[i / 4][i % 4]));
+    if (__any((float)big.x >= vref)) {
+      stay();
+      const float ref = over_groups_max((float)big.x);
+      const float next = fmaxf(vref, __builtin_ldexpf(1.f, __builtin_amdgcn_frexp_expf(ref)));
+      const float f = vref * __builtin_amdgcn_rcpf(next);  // (of a power of two: exact)
       vref = next;
 #pragma unroll
-      for (int n = 0; n < NC; ++n) {
-        lost[n] *= f;
+      for (int n = 0; n < NC; ++n)
 #pragma unroll
         for (int m = 0; m < kRows; ++m) o[n][m] *= f;
-      }
     }
-    const float vinv = 0x1p15f / vref;
+    const float vinv = kWeight * __builtin_amdgcn_rcpf(vref);
     f16x8 p[NC];
 #pragma unroll
-    for (int n = 0; n < NC; ++n) {
-      if (masked)
-        softmax<true>(t, s[n], n, from, vinv, p[n]);
-      else
-        softmax<false>(t, s[n], n, from, vinv, p[n]);
-    }
+    for (int n = 0; n < NC; ++n) weigh<MASK>(s[n], n, from, vinv, p[n]);
+    load_params();
     // pairs of neighbouring keys side by side: 16 bits (4 elements) of each in one word
 #pragma unroll
     for (int half = 0; half < (D == 128 ? 2 : 1); ++half) {
       const uint32_t pick = (D == 128 ? half : c & 1) ? 0x07060302u : 0x05040100u;
       u32x4 x;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        x[i] = __builtin_amdgcn_perm(t.v[i / 2][2 * (i % 2) + 1], t.v[i / 2][2 * (i % 2)], pick);
+      for (int i = 0; i < 4; ++i) x[i] = __builtin_amdgcn_perm(v[i / 2][2 * (i % 2) + 1], v[i / 2][2 * (i % 2)], pick);
       const u32x4 y = x >> 8;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -294,30 +340,36 @@ struct Wave {
           o[n][m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, f), p[n], o[n][m], 0, 0, 0);
       }
     }
+    load_values();
   }
 
-  // Runs over tiles first, first + stride, .. < last.
-  __device__ __forceinline__ void run(int first, int last, int stride, int length, int least_lim, int most_low) {
+  // Runs over tiles first, first + stride, .. < last; all columns see all of the tiles that lie in whole_from ..
+  // whole_to - 1 of the keys.
+  __device__ __forceinline__ void run(int first, int last, int stride, int length, int whole_from, int whole_to) {
     if (first >= last) return;
-    Tile x, y;
-    int i = first;
-    int b0 = block_of(2 * i), b1 = block_of(2 * i + 1);
-    load(x, i, b0, b1);
-    b0 = block_of(2 * (i + stride)), b1 = block_of(2 * (i + stride) + 1);
-    const auto turn = [&](Tile& now, Tile& next) {
-      const int after = i + stride;
-      if (after < last) {
-        load(next, after, b0, b1);
-        b0 = block_of(2 * (after + stride)), b1 = block_of(2 * (after + stride) + 1);
-      }
-      const int from = i * kTile;
-      step(now, from, length, !(from >= most_low && from + kTile <= least_lim));
-      i = after;
+    aim(first, block_of(2 * first), block_of(2 * first + 1));
+    load_keys();
+    load_params();
+    load_values();
+    int next = min(first + stride, last - 1);  // (the last step loads some tile again, which nobody looks at)
+    int b0 = block_of(2 * next), b1 = block_of(2 * next + 1);
+    const auto advance = [&] {
+      aim(next, b0, b1);
+      next = min(next + stride, last - 1);
+      b0 = block_of(2 * next), b1 = block_of(2 * next + 1);
     };
+    const int whole_first = (whole_from + kTile - 1) / kTile, whole_last = min(last, whole_to / kTile);
+    int i = first;
     while (true) {
-      turn(x, y);
+      if (i >= whole_first)
+        for (; i < whole_last; i += stride) {
+          advance();
+          step<false>(i * kTile, length);
+        }
       if (i >= last) break;
-      turn(y, x);
+      advance();
+      step<true>(i * kTile, length);
+      i += stride;
       if (i >= last) break;
     }
   }
@@ -326,12 +378,12 @@ struct Wave {
   template <typename F>
   __device__ __forceinline__ void results(int n, F&& out) {
     constexpr int kEach = kRows;  // neighbouring elements that a lane holds: element kEach (4 g + r) + m
-    const float unit = vref * 0x1p9f, base = over_groups_sum(flat[n] + (kRepair ? 7.5f * 0x1p-15f * vref * lost[n] : 0.f));
+    const float unit = vref * (0x1p24f / kWeight), rest = over_groups_sum(flat[n]);
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       float x[kEach];
 #pragma unroll
-      for (int m = 0; m < kEach; ++m) x[m] = __builtin_fmaf(o[n][m][r], m & 1 ? unit * 0.0625f : unit, base);
+      for (int m = 0; m < kEach; ++m) x[m] = __builtin_fmaf(o[n][m][r], m & 1 ? unit * 0.0625f : unit, rest);
       out(kEach * (4 * g + r), x);
     }
   }
@@ -350,7 +402,7 @@ __device__ void refuse_rows(const AttendArgs& a, const Sequence& s, int kv) {
 // Few queries a sequence: a workgroup of four waves shares the keys of one column tile (or of one of `splits` pieces
 // of them), joined through LDS; pieces are joined by a second kernel.
 template <typename T, int D, int NC>
-__global__ void __launch_bounds__(256) attend_split_kernel(AttendArgs a) {
+__global__ void __launch_bounds__(256, NC == 1 ? 3 : 2) attend_split_kernel(AttendArgs a) {
   constexpr int kCols = 16 * NC;
   __shared__ float part[4][kCols][D + 4];
   __shared__ float maxima[4][kCols], sums[4][kCols];
@@ -373,7 +425,7 @@ __global__ void __launch_bounds__(256) attend_split_kernel(AttendArgs a) {
   const int t0 = first_tile + (int)((long long)max(0, tiles) * split / a.splits);
   const int t1 = first_tile + (int)((long long)max(0, tiles) * (split + 1) / a.splits);
   // (padding columns see nothing: a step that holds some is masked throughout only where the others are)
-  w.run(t0 + wave, t1, 4, s.length, least_lim, most_low);
+  w.run(t0 + wave, t1, 4, s.length, most_low, least_lim);
 
   const int c = w.c;
 #pragma unroll
@@ -385,7 +437,7 @@ __global__ void __launch_bounds__(256) attend_split_kernel(AttendArgs a) {
     });
     const float total = over_groups_sum(w.sum[n]);
     if (w.g == 0) {
-      maxima[wave][16 * n + c] = fmaxf(w.al[n] * w.most[n], -1e38f);  // (finite, whatever the query's size)
+      maxima[wave][16 * n + c] = fmaxf(-w.shift[n], -1e38f);  // (finite, whatever the query's size)
       sums[wave][16 * n + c] = total;
     }
   }
@@ -461,7 +513,7 @@ __global__ void __launch_bounds__(256) attend_join_kernel(AttendArgs a) {
 // Many queries a sequence: each wave has columns of its own and runs over all the keys that they see; the four waves of
 // a workgroup hold neighbouring columns, so that they read the same keys at about the same time.
 template <typename T, int D, int NC>
-__global__ void __launch_bounds__(256) attend_prompt_kernel(AttendArgs a) {
+__global__ void __launch_bounds__(256, 2) attend_prompt_kernel(AttendArgs a) {
   constexpr int kCols = 16 * NC;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int pair = blockIdx.x, b = pair / a.kv_heads, kv = pair - b * a.kv_heads;
@@ -479,7 +531,7 @@ __global__ void __launch_bounds__(256) attend_prompt_kernel(AttendArgs a) {
   const int end = max(0, s.before + last_q + 1), least_lim = max(0, s.before + first_q + 1);
   const int start = a.window > 0 ? max(0, least_lim - a.window) : 0;
   const int most_low = a.window > 0 ? max(0, end - a.window) : 0;
-  w.run(start / kTile, (end + kTile - 1) / kTile, 1, s.length, least_lim, most_low);
+  w.run(start / kTile, (end + kTile - 1) / kTile, 1, s.length, most_low, least_lim);
 #pragma unroll
   for (int n = 0; n < NC; ++n) {
     const float total = over_groups_sum(w.sum[n]);
