@@ -106,7 +106,7 @@ int serving_attend_kv4(const void* query, long long q_token, long long q_head, c
                        void* stream);
 
 /*
- * Of each row of logits [rows, vocab] (type: 0 = fp16, 1 = bf16, 2 = fp32; row stride in elements):
+ * Of each row of logits [rows, vocab] (vocab up to 2096640; type: 0 = fp16, 1 = bf16, 2 = fp32; row stride in elements):
  *   logprob[r]  = x[token_ids[r]] - log sum exp x          (NaN for a token outside the vocabulary)
  *   entropy[r]  = - sum p log p,  p = softmax x            (a logit of -inf adds nothing)
  *   top_ids[r], top_logprobs[r] [rows, top]: the `top` (0 .. 64) most likely tokens, the most likely first, among

@@ -125,7 +125,7 @@ def test_logprobs_refusals(lib):
     assert score(kind=3) == -2 and score(kind=-1) == -2
     assert score(x=ctypes.c_void_p(4097)) == -6 and score(x=ctypes.c_void_p(4098), kind=2) == -6
     assert score(vocab=500000, ws=None) == -9 and score(vocab=500000, ws_bytes=8) == -9
-    assert score(vocab=1 << 30, rows=1 << 20) == -8
+    assert score(vocab=2096641) == -2 and score(vocab=20000, rows=1 << 30) == -8
 
 
 # ---------------------------------------------------------------------------------------------------------------

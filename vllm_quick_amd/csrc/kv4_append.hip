@@ -151,7 +151,10 @@ __global__ void __launch_bounds__(kThreads) rope_append_kernel(AppendArgs a) {
     for (int i = 1; i < 16; ++i) lo = fminf(lo, x[i]), hi = fmaxf(hi, x[i]), nan |= x[i] != x[i];
     if (nan) hi = __builtin_inff();  // (min and max pass a NaN by)
     row_range<L>(lo, hi);
-    f16 least = (f16)lo, scale = (f16)((hi - (float)least) * (1.f / 15.f));
+    f16 least = (f16)lo;
+    float step = (hi - (float)least) * (1.f / 15.f);
+    asm("" : "+v"(step));  // (rounded to fp32 before it is to fp16: one instruction would do both at once)
+    f16 scale = (f16)step;
     const bool held = __builtin_isfinite((float)least) && __builtin_isfinite((float)scale);
     uint32_t wa = 0, wb = 0;
     if (held && (float)scale > 0.f) {

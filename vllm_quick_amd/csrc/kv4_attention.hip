@@ -2,14 +2,16 @@
 // softmax, on 16x16x32 matrix instructions.
 //
 // Codes reach the matrix cores without being converted.  A code n in the low bits of a 16-bit lane IS the fp16 number
-// n 2^-24 (a subnormal; four bits further up 16 n 2^-24), and the matrix instructions take subnormals exactly.  So a
-// word of 8 codes becomes a fragment of 8 fp16 numbers with four ands and a shift, and the scales and leasts of the
-// format stay outside the product:
+// n 2^-24 (a subnormal; four bits further up 16 n 2^-24), which the matrix instructions take.  So a word of 8 codes
+// becomes a fragment of 8 fp16 numbers with four ands and a shift, and the scales and leasts of the format stay outside
+// the product:
 //   q . k_j  =  scale_j (q . code_j) + least_j sum(q)             sum(q) once for each query
 //   o        =  sum_j (p_j vscale_j) code_j + sum_j p_j vleast_j    the second sum is one number for all of a head's
 //                                                                elements
-// Where the sixteens stand in the keys' fragments the queries are divided by 16; in the values' they belong to whole
-// rows of the result.
+// Where the sixteens stand in the keys' fragments the queries are divided by 16.  The values' codes all go in as 16 n
+// (two shifts a word more): a product of n 2^-24 is cut off at some 2^-17 of it, always downwards, which in a long
+// sequence, where the sum of w_j code_j is a hundred times the result, showed as 6e-4 of an fp16 result (26 000 keys);
+// of 16 n 2^-24 a sixteenth of that is cut off.
 //
 // A wave works on 16 NC columns (queries x heads of one kv head) and 32 keys at a time:
 //   S^T = K Q^T   A = codes of 16 keys (lane & 15) x 32 elements, one 16-byte load a lane for a whole head of 128
@@ -18,9 +20,10 @@
 //                  piece, so that the same 4 keys of a piece are again one 16-byte load, and one byte permutation a
 //                  word pairs the codes of neighbouring keys.
 // Roundings: queries enter exactly (scaled by a power of two into fp16's range), w_j = p_j vscale_j is rounded to fp16
-// once, all sums are fp32.  A code stands for zero at n_j = -least_j / vscale_j, not at 0, so w_j's rounding costs
-// (n - n_j) + n_j steps of it; the second part, w_j's error times n_j, is the same for all elements and goes into the
-// second sum (n_j to an eighth).  Only for fp16 results: bf16 ones are rounded coarser than what it repairs.
+// once, all sums are fp32.  For fp16 results the other two sums, of p_j and of p_j vleast_j, take what w_j became divided
+// by vscale_j (to an eighth of the difference) in place of p_j: a rounding then weighs a key by a little more or less, by
+// all elements and the denominator alike, where otherwise it would cost up to 15 steps of the codes.  bf16 results are
+// rounded coarser than that.
 #include "kv4_cache.h"
 
 namespace {
@@ -29,8 +32,9 @@ using namespace serving;
 
 constexpr float kNone = -1e30f;  // below every score, yet finite: differences of it are numbers
 constexpr int kTile = 32;        // keys of a step
+constexpr int kRun = 32;         // steps between two settings aside
 constexpr float kSlack = 8.f;     // a probability may stand this many powers of two above 1 before the maximum moves
-constexpr float kWeight = 0x1p7f;  // p vscale / (power of two above vscale) times this is rounded to fp16: below 2^15
+constexpr float kWeightLog = 7.f;  // p vscale / (power of two above vscale) 2^7 is rounded to fp16: below 2^15
 
 struct AttendArgs {
   const void* query;
@@ -46,7 +50,8 @@ struct AttendArgs {
   int num_blocks, block_size;
   uint32_t per_block_magic;  // ceil(2^32 / (block_size / 16)), or 0 for blocks of 16
   float scale;               // of the scores, times log2(e)
-  int window, max_query_len, splits;
+  int window, max_query_len;
+  int splits, chunk;  // pieces of a sequence, keys of one (the last piece takes what is left)
 };
 
 // Uniform integers that no kernel here writes, through the scalar cache: a vector load would return behind all the
@@ -102,28 +107,45 @@ struct Wave {
   uint32_t k[2][kSteps];
   u32x4 v[2], kp[2], vp[2];
   f16x8 q[NC][kSteps];
-  float qs[NC], al[NC];  // sum of the query, and what makes a score (in powers of two) of a product
+  float qs[NC];          // sum of the query, in the unit of the scores
   int lim[NC], low[NC];  // keys that a column sees: low .. lim - 1
-  float shift[NC];       // p = 2^(al u + shift): no p passes 2^kSlack
+  float shift[NC];       // p 2^weight_log = 2^(score + shift): no p passes 2^kSlack
   float sum[NC], flat[NC];
+  float unit_score;      // what makes a score (in powers of two) of a product
+  float* kept;                        // in LDS: [16 NC][D + 4], what was set aside of the sums of p v,
+  float kept_sum[NC], kept_shift[NC];  // of p, and the shift that both go with
+  bool keeps;
   f32x4 o[NC][kRows];
-  float vref;                // power of two above every vscale so far
+  float vref;                // power of two above every vscale so far,
+  float weight_log;          // and what p's are held at for it: p vscale 2^weight_log is below 2^(kSlack + kWeightLog)
   const uint8_t* head_base;  // of this kv head in block 0
   scalar_ints table;
   long long block_bytes;
   int last_page;
   const uint8_t* base[2];  // where the next step's two groups of 16 tokens are
   int place[2];
-  bool known[2];
+  bool known[2], known_now[2];  // whether the cache has their blocks, and those of the keys in the registers
 
   __device__ __forceinline__ Wave(const AttendArgs& args) : a(args), c(threadIdx.x & 15), g((threadIdx.x & 63) >> 4) {}
 
-  __device__ __forceinline__ void begin(const Sequence& s, int b, int kv, int col0, int cols) {
+  // The first loads, then the queries while they are under way.
+  __device__ __forceinline__ void begin(const Sequence& s, int b, int kv, int col0, int cols, int first, int last, float* lds) {
+    kept = lds;
+    keeps = false;
     head_base = a.cache + (long long)kv * Kv4<D>::block_bytes(a.block_size);
     block_bytes = Kv4<D>::block_bytes(a.block_size) * a.kv_heads;
     table = scalar(a.tables + b * a.table_stride);
     last_page = max(0, page_of((s.length - 1) >> 4));
+    if (first < last) {
+      aim(first, block_of(2 * first), block_of(2 * first + 1));
+      load_keys();
+      load_params();
+      load_values();
+    }
     vref = 0x1p-40f;
+    weight_log = kWeightLog + 40.f;
+    float x[NC][kSteps][8], big = 0.f;
+    const float sign = a.scale < 0.f ? -1.f : 1.f;
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
       const int col = col0 + 16 * n + c;
@@ -133,33 +155,38 @@ struct Wave {
       low[n] = a.window > 0 ? max(0, lim[n] - a.window) : 0;
       const T* src = static_cast<const T*>(a.query) + (long long)(s.row + qi) * a.q_token + (kv * a.group + h) * a.q_head;
       typedef T vec8 __attribute__((ext_vector_type(8)));
-      float x[kSteps][8], big = 0.f, total = 0.f;
+      float most = 0.f, total = 0.f;
 #pragma unroll
       for (int j = 0; j < kSteps; ++j) {
         vec8 w = {};
         if (on) w = *reinterpret_cast<const vec8*>(src + (D / 4) * g + 8 * j);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          x[j][i] = (float)w[i];
-          big = fmaxf(big, fabsf(x[j][i]));
-          total += x[j][i];
+          x[n][j][i] = sign * (float)w[i];
+          most = fmaxf(most, fabsf(x[n][j][i]));
+          total += x[n][j][i];
         }
       }
-      big = over_groups_max(big);
-      total = over_groups_sum(total);
-      // into [2^13, 2^14): a sixteenth of it, and of what is far below it, is still a normal fp16 number
-      const int e = 14 - __builtin_amdgcn_frexp_expf(big);
-      const float sign = a.scale < 0.f ? -1.f : 1.f;
+      qs[n] = over_groups_sum(total);
+      big = fmaxf(big, most < __builtin_inff() ? most : 0.f);  // (an infinite query is its own column's affair)
+    }
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) big = fmaxf(big, __shfl_xor(big, m));
+    // All columns by one power of two, the largest element into [2^13, 2^14): a sixteenth of it, and of what is far below
+    // it, is still a normal fp16 number, and what is not is 2^-38 of the largest score.
+    const int e = 14 - __builtin_amdgcn_frexp_expf(big);
+    unit_score = __builtin_ldexpf(fabsf(a.scale), 24 - e);
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
 #pragma unroll
       for (int j = 0; j < kSteps; ++j) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {  // element (i % 2) * 4 + i / 2 of the word is where the masks leave it
           const int el = (i & 1) * 4 + (i >> 1);
-          q[n][j][i] = (f16)__builtin_ldexpf(sign * x[j][el], (i >> 1) & 1 ? e - 4 : e);
+          q[n][j][i] = (f16)__builtin_ldexpf(x[n][j][el], (i >> 1) & 1 ? e - 4 : e);
         }
       }
-      qs[n] = __builtin_ldexpf(sign * total, e - 24);
-      al[n] = __builtin_ldexpf(fabsf(a.scale), 24 - e);
+      qs[n] = __builtin_ldexpf(qs[n], e - 24) * unit_score;
       shift[n] = -kNone;
       sum[n] = flat[n] = 0.f;
 #pragma unroll
@@ -178,6 +205,7 @@ struct Wave {
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       const int sixteenth = 2 * tile + s, block = s ? block1 : block0;
+      known_now[s] = known[s];
       known[s] = (uint32_t)block < (uint32_t)a.num_blocks;
       const int page = page_of(sixteenth);
       place[s] = page <= last_page ? 16 * sixteenth - page * a.block_size : 0;
@@ -207,8 +235,6 @@ struct Wave {
       const uint32_t at = (uint32_t)(Kv4<D>::key_params(a.block_size) + 4 * place[s]);
       kp[s] = *reinterpret_cast<const u32x4*>(base[s] + at + (uint32_t)(16 * g));
       vp[s] = *reinterpret_cast<const u32x4*>(base[s] + (at + 4 * (uint32_t)a.block_size) + (uint32_t)(16 * g));
-      if (!known[s])  // a block that the cache does not have: its keys are NaN
-        kp[s] = u32x4{0x7e007e00u, 0x7e007e00u, 0x7e007e00u, 0x7e007e00u};
     }
   }
 
@@ -225,58 +251,54 @@ struct Wave {
     return key >= low[n] && key < lim[n];
   }
 
-  // Scores of 32 keys to weights, the B operand of the second product.
+  // Scores of 32 keys to weights, the B operand of the second product.  ks: the keys' scales in the unit of the scores.
   template <bool MASK>
-  __device__ __forceinline__ void weigh(const f32x4 (&s)[2], int n, int from, float vinv, f16x8& p) {
-    float u[8], e[8], w[8], least[8];
+  __device__ __forceinline__ void weigh(const f32x4 (&s)[2], int n, int from, const float (&ks)[8], f16x8& p) {
+    float t[8];
+    const auto score = [&](int i, float more) {
+      return __builtin_fmaf(ks[i], s[i / 4][i % 4], __builtin_fmaf((float)as_pair(kp[i / 4][i % 4]).y, qs[n], more));
+    };
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const f16x2 par = as_pair(kp[i / 4][i % 4]);
-      u[i] = __builtin_fmaf(s[i / 4][i % 4], (float)par.x, (float)par.y * qs[n]);
+      t[i] = score(i, shift[n]);
+      if (MASK) t[i] = sees(n, from, i) ? t[i] : kNone;
     }
-    if (MASK) {
+    float most = t[0];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) u[i] = sees(n, from, i) ? u[i] : kNone;
-    }
-    float most = u[0];
-#pragma unroll
-    for (int i = 1; i < 8; ++i) most = fmaxf(most, u[i]);
-    if (__any(__builtin_fmaf(al[n], most, shift[n]) > kSlack)) {
+    for (int i = 1; i < 8; ++i) most = fmaxf(most, t[i]);
+    if (__any(most > kSlack + weight_log)) {
       stay();
+      most = kNone;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) most = !MASK || sees(n, from, i) ? fmaxf(most, score(i, 0.f)) : most;
       most = over_groups_max(most);  // (a column moves for its own keys only, whatever the wave's others do)
-      const float next = __builtin_fmaf(al[n], most, shift[n]) > kSlack ? -al[n] * most : shift[n];
+      const float next = most + shift[n] > kSlack + weight_log ? weight_log - most : shift[n];
       const float f = exp2_(next - shift[n]);
       shift[n] = next;
       sum[n] *= f;
       flat[n] *= f;
 #pragma unroll
       for (int m = 0; m < kRows; ++m) o[n][m] *= f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {  // (rounded as outside of this branch, which other columns may have called for)
+        t[i] = score(i, next);
+        if (MASK) t[i] = sees(n, from, i) ? t[i] : kNone;
+      }
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const f16x2 par = as_pair(vp[i / 4][i % 4]);
-      e[i] = exp2_(__builtin_fmaf(al[n], u[i], shift[n]));
-      w[i] = e[i] * ((float)par.x * vinv);
-      least[i] = (float)par.y;
-    }
-    if (MASK) {  // (not 0 times what a hidden key's parameters may be)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      float e = exp2_(t[i]), w = e * (float)par.x, least = (float)par.y;
+      if (MASK) {  // (not 0 times what a hidden key's parameters may be)
         const bool on = sees(n, from, i);
-        e[i] = on ? e[i] : 0.f;
-        w[i] = on ? w[i] : 0.f;
-        least[i] = on ? least[i] : 0.f;
+        e = on ? e : 0.f;
+        w = on ? w : 0.f;
+        least = on ? least : 0.f;
       }
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      sum[n] += e[i];
-      flat[n] = __builtin_fmaf(e[i], least[i], flat[n]);
-      p[i] = (f16)w[i];
-      if (kRepair) {
-        const float vs = (float)as_pair(vp[i / 4][i % 4]).x * vinv;
-        flat[n] = __builtin_fmaf((float)p[i] - w[i], least[i] * rough_reciprocal(fmaxf(vs, 0x1p-40f)), flat[n]);
-      }
+      p[i] = (f16)w;
+      if (kRepair) e = __builtin_fmaf((float)p[i] - w, rough_reciprocal(fmaxf((float)par.x, 0x1p-40f)), e);
+      sum[n] += e;
+      flat[n] = __builtin_fmaf(e, least, flat[n]);
     }
   }
 
@@ -309,19 +331,28 @@ struct Wave {
     for (int i = 1; i < 8; ++i) big = __builtin_elementwise_max(big, as_pair(vp[i / 4][i % 4]));
     if (__any((float)big.x >= vref)) {
       stay();
-      const float ref = over_groups_max((float)big.x);
-      const float next = fmaxf(vref, __builtin_ldexpf(1.f, __builtin_amdgcn_frexp_expf(ref)));
-      const float f = vref * __builtin_amdgcn_rcpf(next);  // (of a power of two: exact)
-      vref = next;
+      const int to = __builtin_amdgcn_frexp_expf(over_groups_max((float)big.x));  // 2^to is above every scale
+      const float f = vref * __builtin_ldexpf(1.f, -to), log_f = kWeightLog - (float)to - weight_log;
+      vref = __builtin_ldexpf(1.f, to);
+      weight_log = kWeightLog - (float)to;
 #pragma unroll
-      for (int n = 0; n < NC; ++n)
+      for (int n = 0; n < NC; ++n) {
+        shift[n] = shift[n] >= -kNone ? shift[n] : shift[n] + log_f;
+        sum[n] *= f;
+        flat[n] *= f;
 #pragma unroll
         for (int m = 0; m < kRows; ++m) o[n][m] *= f;
+      }
     }
-    const float vinv = kWeight * __builtin_amdgcn_rcpf(vref);
+    float ks[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      ks[i] = (float)as_pair(kp[i / 4][i % 4]).x * unit_score;
+      if (MASK && !known_now[i / 4]) ks[i] = __builtin_nanf("");  // of a block that the cache does not have
+    }
     f16x8 p[NC];
 #pragma unroll
-    for (int n = 0; n < NC; ++n) weigh<MASK>(s[n], n, from, vinv, p[n]);
+    for (int n = 0; n < NC; ++n) weigh<MASK>(s[n], n, from, ks, p[n]);
     load_params();
     // pairs of neighbouring keys side by side: 16 bits (4 elements) of each in one word
 #pragma unroll
@@ -330,10 +361,9 @@ struct Wave {
       u32x4 x;
 #pragma unroll
       for (int i = 0; i < 4; ++i) x[i] = __builtin_amdgcn_perm(v[i / 2][2 * (i % 2) + 1], v[i / 2][2 * (i % 2)], pick);
-      const u32x4 y = x >> 8;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const u32x4 f = (e & 2 ? y : x) & (e & 1 ? 0x00f000f0u : 0x000f000fu);
+        const u32x4 f = (e == 0 ? x << 4 : e == 1 ? x : e == 2 ? x >> 4 : x >> 8) & 0x00f000f0u;
         const int m = 4 * half + e;
 #pragma unroll
         for (int n = 0; n < NC; ++n)
@@ -343,14 +373,10 @@ struct Wave {
     load_values();
   }
 
-  // Runs over tiles first, first + stride, .. < last; all columns see all of the tiles that lie in whole_from ..
+  // Runs over tiles first, first + stride, .. < last, the first of them loaded by begin(); all columns see all of the tiles that lie in whole_from ..
   // whole_to - 1 of the keys.
   __device__ __forceinline__ void run(int first, int last, int stride, int length, int whole_from, int whole_to) {
     if (first >= last) return;
-    aim(first, block_of(2 * first), block_of(2 * first + 1));
-    load_keys();
-    load_params();
-    load_values();
     int next = min(first + stride, last - 1);  // (the last step loads some tile again, which nobody looks at)
     int b0 = block_of(2 * next), b1 = block_of(2 * next + 1);
     const auto advance = [&] {
@@ -361,11 +387,17 @@ struct Wave {
     const int whole_first = (whole_from + kTile - 1) / kTile, whole_last = min(last, whole_to / kTile);
     int i = first;
     while (true) {
-      if (i >= whole_first)
-        for (; i < whole_last; i += stride) {
+      if (i >= whole_first) {
+        const int stop = min(whole_last, i + kRun * stride);
+        for (; i < stop && known[0] && known[1]; i += stride) {
           advance();
           step<false>(i * kTile, length);
         }
+        if (i >= stop && i < whole_last) {
+          set_aside();
+          continue;
+        }
+      }
       if (i >= last) break;
       advance();
       step<true>(i * kTile, length);
@@ -374,20 +406,61 @@ struct Wave {
     }
   }
 
-  // Element d of the result of this lane's column, as sums of p v: out(piece of kEach elements, first element, values).
+  // Adds what the registers hold to what LDS keeps, and begins anew.  The codes are not centred, so that the two sums
+  // that make a result are many times larger than it, the more so the longer the sequence: over 60 000 keys of one wave
+  // fp16 results are 2.9e-4 off with this, 6.9e-4 without.  Each lane has places of its own: no barrier.
+  __device__ __forceinline__ void set_aside() {
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+      const float f = keeps ? exp2_(shift[n] - kept_shift[n]) : 0.f;
+      kept_sum[n] = keeps ? __builtin_fmaf(kept_sum[n], f, sum[n]) : sum[n];
+      kept_shift[n] = shift[n];
+      results(n, [&](int d, const float* x) {
+        f32x4* at = reinterpret_cast<f32x4*>(kept + (16 * n + c) * (D + 4) + d);
+#pragma unroll
+        for (int m = 0; m < kRows; m += 4) {
+          f32x4 y = {x[m], x[m + 1], x[m + 2], x[m + 3]};
+          if (keeps) y += at[m / 4] * f;
+          at[m / 4] = y;
+        }
+      });
+      sum[n] = flat[n] = 0.f;
+#pragma unroll
+      for (int m = 0; m < kRows; ++m) o[n][m] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    keeps = true;
+  }
+
+  // Element d of the result of this lane's column, as sums of p v 2^weight_log: out(piece of kEach elements, first element, values).
   template <typename F>
   __device__ __forceinline__ void results(int n, F&& out) {
     constexpr int kEach = kRows;  // neighbouring elements that a lane holds: element kEach (4 g + r) + m
-    const float unit = vref * (0x1p24f / kWeight), rest = over_groups_sum(flat[n]);
+    const float rest = over_groups_sum(flat[n]);
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       float x[kEach];
 #pragma unroll
-      for (int m = 0; m < kEach; ++m) x[m] = __builtin_fmaf(o[n][m][r], m & 1 ? unit * 0.0625f : unit, rest);
+      for (int m = 0; m < kEach; ++m) x[m] = __builtin_fmaf(o[n][m][r], 0x1p20f, rest);
       out(kEach * (4 * g + r), x);
     }
   }
 };
+
+// Keys that columns first .. last of a tile see (some of them: tiles first_tile .. last_tile - 1; all: keys whole_from
+// .. whole_to - 1).
+struct Range {
+  int first_tile, last_tile, whole_from, whole_to;
+};
+__device__ __forceinline__ Range range(const AttendArgs& a, const Sequence& s, int first, int last) {
+  const int end = max(0, s.before + last / a.group + 1), whole_to = max(0, s.before + first / a.group + 1);
+  const int start = a.window > 0 ? max(0, whole_to - a.window) : 0;
+  return Range{start / kTile, (end + kTile - 1) / kTile, a.window > 0 ? max(0, end - a.window) : 0, whole_to};
+}
+// How many pieces they come in: as many as a sequence of this length needs, at most `splits`.
+__device__ __forceinline__ int pieces_of(const AttendArgs& a, const Range& r) {
+  const int per_piece = a.chunk / kTile;
+  return max(1, min(a.splits, (r.last_tile - r.first_tile + per_piece - 1) / per_piece));
+}
 
 // The rows of a sequence past max_query_len were promised not to exist: they say so.
 template <typename T, int D>
@@ -399,13 +472,13 @@ __device__ void refuse_rows(const AttendArgs& a, const Sequence& s, int kv) {
   }
 }
 
-// Few queries a sequence: a workgroup of four waves shares the keys of one column tile (or of one of `splits` pieces
+// Few queries a sequence: the waves of a workgroup share the keys of one column tile (or of one of `splits` pieces
 // of them), joined through LDS; pieces are joined by a second kernel.
-template <typename T, int D, int NC>
-__global__ void __launch_bounds__(256, NC == 1 ? 3 : 2) attend_split_kernel(AttendArgs a) {
+template <typename T, int D, int NC, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES, NC == 1 ? 3 : 2) attend_split_kernel(AttendArgs a) {
   constexpr int kCols = 16 * NC;
-  __shared__ float part[4][kCols][D + 4];
-  __shared__ float maxima[4][kCols], sums[4][kCols];
+  __shared__ float part[WAVES][kCols][D + 4];
+  __shared__ float maxima[WAVES][kCols], sums[WAVES][kCols];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int pair = blockIdx.x, b = pair / a.kv_heads, kv = pair - b * a.kv_heads;
   const int split = blockIdx.y, tile = blockIdx.z;
@@ -414,44 +487,36 @@ __global__ void __launch_bounds__(256, NC == 1 ? 3 : 2) attend_split_kernel(Atte
   if (tile == 0 && split == 0 && queries < s.queries) refuse_rows<T, D>(a, s, kv);
   const int col0 = tile * kCols;
   if (col0 >= cols) return;
+  const Range r = range(a, s, col0, min(cols - 1, col0 + kCols - 1));
+  const int pieces = pieces_of(a, r);
+  if (split >= pieces) return;
+  const int per_piece = a.chunk / kTile;
+  const int t0 = r.first_tile + split * per_piece + wave;
+  const int t1 = split == pieces - 1 ? r.last_tile : r.first_tile + (split + 1) * per_piece;
   Wave<T, D, NC> w(a);
-  w.begin(s, b, kv, col0, cols);
-  const int first_q = col0 / a.group, last_q = min(cols - 1, col0 + kCols - 1) / a.group;
-  const int end = max(0, s.before + last_q + 1);            // keys that any column sees end here
-  const int least_lim = max(0, s.before + first_q + 1);     // and those that all see, here
-  const int start = a.window > 0 ? max(0, least_lim - a.window) : 0;
-  const int most_low = a.window > 0 ? max(0, end - a.window) : 0;
-  const int first_tile = start / kTile, tiles = (end + kTile - 1) / kTile - first_tile;
-  const int t0 = first_tile + (int)((long long)max(0, tiles) * split / a.splits);
-  const int t1 = first_tile + (int)((long long)max(0, tiles) * (split + 1) / a.splits);
-  // (padding columns see nothing: a step that holds some is masked throughout only where the others are)
-  w.run(t0 + wave, t1, 4, s.length, most_low, least_lim);
+  w.begin(s, b, kv, col0, cols, t0, t1, &part[wave][0][0]);
+  w.run(t0, t1, WAVES, s.length, r.whole_from, r.whole_to);
 
-  const int c = w.c;
+  w.set_aside();
 #pragma unroll
   for (int n = 0; n < NC; ++n) {
-    w.results(n, [&](int d, const float* x) {
-#pragma unroll
-      for (int m = 0; m < D / 16; m += 4)
-        *reinterpret_cast<f32x4*>(&part[wave][16 * n + c][d + m]) = f32x4{x[m], x[m + 1], x[m + 2], x[m + 3]};
-    });
-    const float total = over_groups_sum(w.sum[n]);
+    const float total = over_groups_sum(w.kept_sum[n]);
     if (w.g == 0) {
-      maxima[wave][16 * n + c] = fmaxf(-w.shift[n], -1e38f);  // (finite, whatever the query's size)
-      sums[wave][16 * n + c] = total;
+      maxima[wave][16 * n + w.c] = -w.shift[n];
+      sums[wave][16 * n + w.c] = total;
     }
   }
   __syncthreads();
-  constexpr int kEach = D * kCols / 256;  // elements of a column that a thread joins
+  constexpr int kEach = D * kCols / (64 * WAVES);  // elements of a column that a thread joins
   constexpr int kPer = D / kEach;
   const int col = threadIdx.x / kPer, d0 = (threadIdx.x % kPer) * kEach;
   if (col0 + col >= cols) return;
   float top = maxima[0][col];
 #pragma unroll
-  for (int i = 1; i < 4; ++i) top = fmaxf(top, maxima[i][col]);
+  for (int i = 1; i < WAVES; ++i) top = fmaxf(top, maxima[i][col]);
   float total = 0.f, x[kEach] = {};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < WAVES; ++i) {
     const float f = exp2_(maxima[i][col] - top);
     total = __builtin_fmaf(sums[i][col], f, total);
 #pragma unroll
@@ -459,7 +524,7 @@ __global__ void __launch_bounds__(256, NC == 1 ? 3 : 2) attend_split_kernel(Atte
   }
   const int qi = (col0 + col) / a.group, head = kv * a.group + (col0 + col) - qi * a.group;
   const long long at = (long long)(s.row + qi) * a.heads + head;
-  if (a.splits == 1) {
+  if (pieces == 1) {
     const float inv = total == 0.f ? 0.f : 1.f / total;
     T* dst = static_cast<T*>(a.out) + at * D + d0;
 #pragma unroll
@@ -476,38 +541,75 @@ __global__ void __launch_bounds__(256, NC == 1 ? 3 : 2) attend_split_kernel(Atte
   }
 }
 
-// Joins the pieces of a query head: one wave each.
-template <typename T, int D>
+// Joins the pieces of a query head: one wave each, a lane a piece for the factors, then 16 bytes a lane of several
+// pieces at once.
+template <typename T, int D, int NC>
 __global__ void __launch_bounds__(256) attend_join_kernel(AttendArgs a) {
-  const long long at = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (at >= (long long)a.tokens * a.heads) return;
-  const int row = (int)(at / a.heads);
-  if (a.query_start) {  // rows of no sequence stay as they are, rows past max_query_len too: the first kernel wrote them
-    int lo = 0, hi = a.seqs;  // the last sequence that begins at or before this row
+  const int at = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (at >= a.tokens * a.heads) return;
+  const int row = at / a.heads, kv = (at - row * a.heads) / a.group;
+  int b = row;
+  if (a.query_start) {  // the last sequence that begins at or before this row
+    int lo = 0, hi = a.seqs;
     while (hi - lo > 1) {
       const int mid = (lo + hi) / 2;
-      if (a.query_start[mid] <= row)
+      if (scalar(a.query_start)[mid] <= row)
         lo = mid;
       else
         hi = mid;
     }
-    if (row < a.query_start[lo] || row >= min(a.query_start[lo + 1], a.query_start[lo] + a.max_query_len)) return;
+    b = lo;
   }
+  const Sequence s = sequence(a, b);
+  const int qi = row - s.row, queries = min(s.queries, a.max_query_len);
+  if (qi < 0 || qi >= queries) return;  // a row of no sequence, or one past max_query_len: neither is written here
+  const int cols = queries * a.group, col = qi * a.group + (at - row * a.heads) - kv * a.group;
+  const int col0 = col / (16 * NC) * (16 * NC);
+  const int pieces = pieces_of(a, range(a, s, col0, min(cols - 1, col0 + 16 * NC - 1)));
+  if (pieces == 1) return;  // written by the first kernel
+  constexpr int kLanes = D / 4, kAtOnce = 64 / kLanes;
+  const int lane = threadIdx.x & 63, part = lane / kLanes, d = 4 * (lane % kLanes);
+  const float* ml = a.part_ml + (long long)at * a.splits * 2;
+  float most = -1e38f, total = 0.f;
+  if (lane < pieces) most = ml[2 * lane], total = ml[2 * lane + 1];
+  float top = most;
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) top = fmaxf(top, __shfl_xor(top, m));
+  const float f = lane < pieces ? exp2_(most - top) : 0.f;
+  total *= f;
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) total += __shfl_xor(total, m);
+  const float* src = a.part_o + (long long)at * a.splits * D + d;
+  f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+  for (int i = 0; i < pieces; i += kAtOnce) {
+    const int piece = i + part;
+    const float fp = __shfl(f, piece & 63);
+    if (piece < pieces) x += *reinterpret_cast<const f32x4*>(src + (long long)piece * D) * fp;
+  }
+#pragma unroll
+  for (int m = kLanes; m < 64; m <<= 1)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] += __shfl_xor(x[i], m);
+  if (part) return;
+  typedef T vec4 __attribute__((ext_vector_type(4)));
+  vec4 y;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) y[i] = (T)(total == 0.f ? 0.f : x[i] / total);
+  *reinterpret_cast<vec4*>(static_cast<T*>(a.out) + (long long)at * D + d) = y;
+}
+
+// The sequence of the rank'th greatest length, of up to 64 (more fill the chip however they come).
+__device__ __forceinline__ int by_length(const AttendArgs& a, int rank) {
+  if (a.seqs > 64) return rank;
   const int lane = threadIdx.x & 63;
-  const float* ml = a.part_ml + at * a.splits * 2;
-  float top = -1e38f;
-  for (int s = 0; s < a.splits; ++s) top = fmaxf(top, ml[2 * s]);
-  float total = 0.f, x[D / 64] = {};
-  for (int s = 0; s < a.splits; ++s) {
-    const float f = exp2_(ml[2 * s] - top);
-    total = __builtin_fmaf(ml[2 * s + 1], f, total);
-    const float* src = a.part_o + (at * a.splits + s) * D + lane * (D / 64);
-#pragma unroll
-    for (int d = 0; d < D / 64; ++d) x[d] = __builtin_fmaf(src[d], f, x[d]);
+  const int own = lane < a.seqs ? a.seq_lens[lane] : -0x7fffffff;
+  int ahead = 0;
+  for (int i = 0; i < a.seqs; ++i) {
+    const int other = __builtin_amdgcn_readlane(own, i);
+    ahead += other > own || (other == own && i < lane);
   }
-  T* dst = static_cast<T*>(a.out) + at * D + lane * (D / 64);
-#pragma unroll
-  for (int d = 0; d < D / 64; ++d) dst[d] = (T)(total == 0.f ? 0.f : x[d] / total);
+  return __builtin_ctzll(__ballot(ahead == rank && lane < a.seqs));
 }
 
 // Many queries a sequence: each wave has columns of its own and runs over all the keys that they see; the four waves of
@@ -515,8 +617,9 @@ __global__ void __launch_bounds__(256) attend_join_kernel(AttendArgs a) {
 template <typename T, int D, int NC>
 __global__ void __launch_bounds__(256, 2) attend_prompt_kernel(AttendArgs a) {
   constexpr int kCols = 16 * NC;
+  __shared__ float part[4][kCols][D + 4];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int pair = blockIdx.x, b = pair / a.kv_heads, kv = pair - b * a.kv_heads;
+  const int kv = blockIdx.x, b = by_length(a, blockIdx.z);
   const Sequence s = sequence(a, b);
   const int queries = min(s.queries, a.max_query_len), cols = queries * a.group;
   if (blockIdx.y == 0 && queries < s.queries) refuse_rows<T, D>(a, s, kv);
@@ -525,21 +628,24 @@ __global__ void __launch_bounds__(256, 2) attend_prompt_kernel(AttendArgs a) {
   // the columns that see most come first: what is left at the end is short
   const int col0 = (groups - 1 - (int)blockIdx.y) * group_cols + wave * kCols;
   if (col0 >= cols) return;
+  const Range r = range(a, s, col0, min(cols - 1, col0 + kCols - 1));
   Wave<T, D, NC> w(a);
-  w.begin(s, b, kv, col0, cols);
-  const int first_q = col0 / a.group, last_q = min(cols - 1, col0 + kCols - 1) / a.group;
-  const int end = max(0, s.before + last_q + 1), least_lim = max(0, s.before + first_q + 1);
-  const int start = a.window > 0 ? max(0, least_lim - a.window) : 0;
-  const int most_low = a.window > 0 ? max(0, end - a.window) : 0;
-  w.run(start / kTile, (end + kTile - 1) / kTile, 1, s.length, most_low, least_lim);
+  w.begin(s, b, kv, col0, cols, r.first_tile, r.last_tile, &part[wave][0][0]);
+  w.run(r.first_tile, r.last_tile, 1, s.length, r.whole_from, r.whole_to);
+  if (w.keeps) w.set_aside();
 #pragma unroll
   for (int n = 0; n < NC; ++n) {
-    const float total = over_groups_sum(w.sum[n]);
+    const float total = over_groups_sum(w.keeps ? w.kept_sum[n] : w.sum[n]);
     const int col = col0 + 16 * n + w.c;
     const int qi = col / a.group, head = kv * a.group + col - qi * a.group;
     const float inv = total == 0.f ? 0.f : 1.f / total;
-    w.results(n, [&](int d, const float* x) {
+    w.results(n, [&](int d, float* x) {
       if (col >= cols) return;
+      if (w.keeps) {  // (the registers were set aside and hold nothing)
+        const f32x4* at = reinterpret_cast<const f32x4*>(&part[wave][16 * n + w.c][d]);
+#pragma unroll
+        for (int m = 0; m < D / 16; ++m) x[m] = at[m / 4][m % 4];
+      }
       typedef T piece __attribute__((ext_vector_type(D / 16)));
       piece y;
 #pragma unroll
@@ -552,7 +658,7 @@ __global__ void __launch_bounds__(256, 2) attend_prompt_kernel(AttendArgs a) {
 // How a call is laid over the chip, from its sizes alone.
 struct Plan {
   bool prompt;
-  int nc, tiles, splits;
+  int nc, tiles, waves, splits, chunk;
 };
 Plan plan(int seqs, int heads, int kv_heads, int max_query_len, int max_seq_len, int window) {
   const long long cols = (long long)max_query_len * (heads / kv_heads);
@@ -560,15 +666,25 @@ Plan plan(int seqs, int heads, int kv_heads, int max_query_len, int max_seq_len,
   p.prompt = cols > 64;
   p.nc = cols > 16 ? 2 : 1;
   p.tiles = (int)((cols + 16 * p.nc - 1) / (16 * p.nc));
+  p.waves = 4;
   p.splits = 1;
+  p.chunk = 1 << 27;
   if (p.prompt) return p;
   const long long groups = (long long)seqs * kv_heads * p.tiles;
   long long keys = max_seq_len;
-  if (window > 0 && window + max_query_len < keys) keys = window + max_query_len;
-  const long long most = (keys + 511) / 512;  // four waves with four tiles each
-  long long splits = (1024 + groups - 1) / groups;
+  if (window > 0 && (long long)window + max_query_len < keys) keys = window + max_query_len;
+  // Where a workgroup a CU is all there is, eight waves share up to 2048 keys and no second kernel runs: 16 x 4 kv heads
+  // x 1029 keys of 64 take 11.8 us so, 14.6 with four waves and two pieces.  Otherwise as many pieces as fill the chip
+  // once (three workgroups of four waves a CU): 8 x 8 kv heads x 65536 keys of 128 take 90 us in 12 pieces, 104 in 24
+  // (the last round of workgroups leaves most CUs idle), 115 in 48.
+  if (groups * ((keys + 2047) / 2048) <= 256) p.waves = 8;
+  const long long least = p.waves == 8 ? 2048 : 512, most = (keys + least - 1) / least;
+  long long splits = (p.waves == 8 ? 256 : 768) / groups;
   splits = splits < most ? splits : most;
-  p.splits = (int)(splits < 1 ? 1 : splits > 256 ? 256 : splits);
+  splits = splits < 1 ? 1 : splits > 64 ? 64 : splits;
+  if (splits == 1) return p;
+  p.chunk = (int)(((keys + splits - 1) / splits + 127) / 128 * 128);
+  p.splits = (int)((keys + p.chunk - 1) / p.chunk);
   return p;
 }
 
@@ -576,19 +692,29 @@ template <typename T, int D>
 int launch(const AttendArgs& a, const Plan& p, hipStream_t s) {
   const unsigned pairs = (unsigned)a.seqs * (unsigned)a.kv_heads;
   if (p.prompt) {
-    const dim3 grid(pairs, (unsigned)((p.tiles + 3) / 4));
+    // the longest sequence first, and of each the columns that see most: the short ones fill the end.  In one order for
+    // all, 2 x 2048 queries that see up to 2500 and 8192 keys leave 40 % of the CUs' time unused.  A kv head's workgroups
+    // follow each other at a distance of kv_heads, which puts them on the same XCD where that is 8.
+    const dim3 grid((unsigned)a.kv_heads, (unsigned)((p.tiles + 3) / 4), (unsigned)a.seqs);
     hipLaunchKernelGGL((attend_prompt_kernel<T, D, 2>), grid, dim3(256), 0, s, a);
     return serving_after_launch();
   }
   const dim3 grid(pairs, (unsigned)p.splits, (unsigned)p.tiles);
-  if (p.nc == 1)
-    hipLaunchKernelGGL((attend_split_kernel<T, D, 1>), grid, dim3(256), 0, s, a);
+  if (p.nc == 1 && p.waves == 4)
+    hipLaunchKernelGGL((attend_split_kernel<T, D, 1, 4>), grid, dim3(256), 0, s, a);
+  else if (p.nc == 1)
+    hipLaunchKernelGGL((attend_split_kernel<T, D, 1, 8>), grid, dim3(512), 0, s, a);
+  else if (p.waves == 4)
+    hipLaunchKernelGGL((attend_split_kernel<T, D, 2, 4>), grid, dim3(256), 0, s, a);
   else
-    hipLaunchKernelGGL((attend_split_kernel<T, D, 2>), grid, dim3(256), 0, s, a);
+    hipLaunchKernelGGL((attend_split_kernel<T, D, 2, 8>), grid, dim3(512), 0, s, a);
   int rc = serving_after_launch();
   if (rc != SERVING_OK || p.splits == 1) return rc;
-  const long long rows = (long long)a.tokens * a.heads;
-  hipLaunchKernelGGL((attend_join_kernel<T, D>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a);
+  const dim3 join((unsigned)(((long long)a.tokens * a.heads + 3) / 4));
+  if (p.nc == 1)
+    hipLaunchKernelGGL((attend_join_kernel<T, D, 1>), join, dim3(256), 0, s, a);
+  else
+    hipLaunchKernelGGL((attend_join_kernel<T, D, 2>), join, dim3(256), 0, s, a);
   return serving_after_launch();
 }
 
@@ -625,14 +751,14 @@ extern "C" int serving_attend_kv4(const void* query, long long q_token, long lon
   const size_t need = serving_attend_kv4_workspace_bytes(tokens, seqs, heads, kv_heads, head_size, max_query_len, max_seq_len, window);
   if (need && (!workspace || workspace_bytes < need)) return SERVING_E_WORKSPACE;
   if (need && !aligned16(workspace)) return SERVING_E_ALIGN;
-  if ((long long)seqs * kv_heads > 0x7fffffLL || p.tiles > 4 * 65535LL || (long long)tokens * heads > (1LL << 33))
+  if ((long long)seqs * kv_heads > 0x7fffffLL || (p.prompt && seqs > 65535) || p.tiles > 4 * 65535LL || (long long)tokens * heads > 0x7fffffffLL)
     return SERVING_E_TOO_LARGE;
   const int sixteens = block_size / 16;
   AttendArgs a{query, q_token, q_head, static_cast<const uint8_t*>(cache), tables, table_stride, seq_lens, query_start, out,
                static_cast<float*>(workspace), nullptr, table_width, tokens, seqs, heads, kv_heads, heads / kv_heads,
                (int)num_blocks, block_size,
                sixteens == 1 ? 0u : (uint32_t)(((1ULL << 32) + sixteens - 1) / sixteens),
-               scale * 1.44269504088896340736f, window, max_query_len, p.splits};
+               scale * 1.44269504088896340736f, window, max_query_len, p.splits, p.chunk};
   if (need) a.part_ml = a.part_o + (size_t)tokens * heads * p.splits * head_size;
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (head_size == 64) return bf16_in ? launch<bf16, 64>(a, p, s) : launch<f16, 64>(a, p, s);

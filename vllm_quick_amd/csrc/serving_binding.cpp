@@ -235,7 +235,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> token_logprobs(const Tensor& logits, 
   need(token_ids.dim() == 1 && token_ids.size(0) == rows, what, "token_ids must be [rows], got " + shape_of(token_ids));
   need(top_n >= 0 && top_n <= 64 && top_n <= vocab, what,
        "top_n must be from 0 to 64 and no more than the vocabulary, got " + std::to_string(top_n));
-  need(rows <= kMostInt && vocab <= (1 << 30), what, "too many logits");
+  need(rows <= kMostInt && vocab <= 64 * 32760, what, "a vocabulary has at most 2096640 tokens, and there are too many rows or tokens here");
   on_gpu(logits, logits, what, "logits");
   on_gpu(token_ids, logits, what, "token_ids");
   no_gradient(logits, what, "logits");

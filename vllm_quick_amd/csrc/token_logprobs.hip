@@ -18,6 +18,8 @@ using namespace serving;
 constexpr int kMaxTop = 64;       // groups that are ranked for the bound
 constexpr int kCandidates = 1024;  // elements not below the bound that LDS takes; more (rows of equals) go the long way
 
+constexpr int kMaxVocab = 64 * 32760;  // 64 segments: a lane of the join each, and their keys in LDS
+
 typedef unsigned long long u64;
 
 // What a segment leaves of itself for the join: its maximum, how often it occurs, the sums without it.
@@ -98,6 +100,7 @@ __global__ void __launch_bounds__(THREADS, 4) logprobs_kernel(Args a) {
   __shared__ u64 candidates[kCandidates];
   __shared__ u64 wave_best[kWaves];
   __shared__ int n_candidates;
+  __shared__ uint32_t shared_bound;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int row = blockIdx.x / a.segments, seg = blockIdx.x - row * a.segments;
   const int begin = seg * a.segment;                         // of this segment in its row
@@ -178,28 +181,44 @@ __global__ void __launch_bounds__(THREADS, 4) logprobs_kernel(Args a) {
   count = wave_all(count, [](int p, int q) { return p + q; });
   if (lane == 0) sums[wave][0] = rest, sums[wave][1] = weighted, counts[wave] = count;
 
-  // the n-th largest group maximum: each lane counts the groups ahead of its own
-  if (a.top > 0) {
-    int ahead = 0;
-#pragma unroll 16
-    for (int g = 0; g < 64; ++g) {
-      const uint32_t other = __builtin_amdgcn_readlane(group, g);
-      ahead += other > group || (other == group && g < lane);
-    }
-    const uint32_t bound = __builtin_amdgcn_readlane(group, __builtin_ctzll(__ballot(ahead == a.top - 1)));
-    if (ordered(mine) >= bound) {
+  // the n-th largest group maximum: each lane of the last wave counts the groups ahead of its own (told apart by the
+  // lane in the last six bits; what these held only lowers the bound)
+  if (a.top > 0 && wave == kWaves - 1) {
+    const uint32_t own = (group & ~63u) | (uint32_t)(63 - lane);
+    uint32_t ahead = 0;
 #pragma unroll
-      for (int k = 0; k < NV; ++k) {
-        const int e = (k * THREADS + tid) * X::kEach - skip;
+    for (int g = 0; g < 64; ++g) ahead += (uint32_t)__builtin_amdgcn_readlane(own, g) > own ? 1u : 0u;
+    if (ahead == (uint32_t)a.top - 1) shared_bound = group & ~63u;
+  }
+  __syncthreads();
+  if (a.top > 0) {
+    const uint32_t bound = shared_bound;
+    const float border = bound < ordered(-__builtin_inff()) ? -__builtin_inff() : unordered(bound);
+    if (most != most) {  // a row with a NaN: ordered numbers know where it stands, comparisons do not
+#pragma unroll
+      for (int k = 0; k < NV; ++k)
+        for (int i = 0; i < X::kEach; ++i) {
+          const float x = X::get(v[k], i);
+          const int e = (k * THREADS + tid) * X::kEach - skip + i;
+          if (ordered(x) >= bound && e >= 0 && e < size) {
+            const int at = atomicAdd(&n_candidates, 1);
+            if (at < kCandidates) candidates[at] = key_of(x, begin + e);
+          }
+        }
+    } else if (mine >= border) {
+#pragma unroll
+      for (int k = 0; k < NV; ++k)
 #pragma unroll
         for (int i = 0; i < X::kEach; ++i) {
           const float x = X::get(v[k], i);
-          if (ordered(x) >= bound && e + i >= 0 && e + i < size) {
-            const int at = atomicAdd(&n_candidates, 1);
-            if (at < kCandidates) candidates[at] = key_of(x, begin + e + i);
+          if (x >= border) {
+            const int e = (k * THREADS + tid) * X::kEach - skip + i;
+            if (e >= 0 && e < size) {
+              const int at = atomicAdd(&n_candidates, 1);
+              if (at < kCandidates) candidates[at] = key_of(x, begin + e);
+            }
           }
         }
-      }
     }
   }
   __syncthreads();
@@ -267,56 +286,50 @@ __global__ void __launch_bounds__(THREADS, 4) logprobs_kernel(Args a) {
   }
 }
 
-// Joins the segments of a row.
+// Joins the segments of a row: sums by one wave, a lane a segment, the most likely tokens by counting the keys ahead
+// of each.
+constexpr int kJoinKeys = 4096;
+
 template <int TYPE>
 __global__ void __launch_bounds__(256) join_kernel(Args a) {
   typedef Logits<TYPE> X;
   __shared__ double shared_log_z;
   __shared__ float shared_most;
+  __shared__ u64 keys[kJoinKeys];
   const int row = blockIdx.x, tid = threadIdx.x;
   const Part* parts = a.parts + (long long)row * a.segments;
-  const u64* keys = a.keys + (long long)row * a.segments * a.top;
+  const int n = a.segments * a.top;
+  for (int i = tid; i < n; i += 256) keys[i] = a.keys[(long long)row * n + i];
   if (tid < 64) {
-    float most = -__builtin_inff();
-    for (int s = tid; s < a.segments; s += 64) most = larger(most, parts[s].most);
-    most = wave_all(most, [](float p, float q) { return larger(p, q); });
-    double rest = 0.0, weighted = 0.0, count = 0.0;
-    if (__builtin_isfinite(most)) {
-      for (int s = tid; s < a.segments; s += 64) {
-        const Part p = parts[s];
-        if (p.most == most) {
-          count += p.count;
-          rest += p.rest;
-          weighted += p.weighted;
-        } else if (p.most > -__builtin_inff()) {
-          const double d = (double)p.most - (double)most, f = exp(d), z = (double)p.count + p.rest;
-          rest += z * f;
-          weighted += (p.weighted + z * d) * f;
-        }
-      }
+    const long long token = a.token_ids[row];
+    const bool known = token >= 0 && token < a.vocab;
+    const uint8_t* p = a.logits + row * a.row_stride + (known ? token : 0) * X::kBytes;
+    const float x = TYPE == 2 ? *reinterpret_cast<const float*>(p)
+                    : TYPE == 1 ? __builtin_bit_cast(float, (uint32_t)*reinterpret_cast<const uint16_t*>(p) << 16)
+                                : (float)*reinterpret_cast<const f16*>(p);
+    Part own = {-__builtin_inff(), 0.f, 0.f, 0};
+    if (tid < a.segments) own = parts[tid];
+    const float most = wave_all(own.most, [](float p, float q) { return larger(p, q); });
+    float rest = 0.f, weighted = 0.f, count = 0.f;
+    if (own.most == most) {
+      count = (float)own.count, rest = own.rest, weighted = own.weighted;
+    } else if (own.most > -__builtin_inff()) {
+      const float d = own.most - most, f = __builtin_amdgcn_exp2f(d * 1.44269504088896340736f), z = (float)own.count + own.rest;
+      rest = z * f;
+      weighted = __builtin_fmaf(z, d, own.weighted) * f;
     }
-    const auto add = [](double p, double q) { return p + q; };
+    const auto add = [](float p, float q) { return p + q; };
     rest = wave_all(rest, add), weighted = wave_all(weighted, add), count = wave_all(count, add);
     double log_z = __builtin_nan(""), entropy = __builtin_nan("");
     if (__builtin_isfinite(most)) finish(count, rest, weighted, log_z, entropy);
     if (tid == 0) {
       shared_log_z = log_z;
       shared_most = most;
-      const long long token = a.token_ids[row];
-      float lp = __builtin_nanf("");
-      if (token >= 0 && token < a.vocab) {
-        const uint8_t* p = a.logits + row * a.row_stride + token * X::kBytes;
-        const float x = TYPE == 2 ? *reinterpret_cast<const float*>(p)
-                        : TYPE == 1 ? __builtin_bit_cast(float, (uint32_t)*reinterpret_cast<const uint16_t*>(p) << 16)
-                                    : (float)*reinterpret_cast<const f16*>(p);
-        lp = (float)((double)(x - most) - log_z);
-      }
-      a.logprob[row] = lp;
+      a.logprob[row] = known ? (float)((double)(x - most) - log_z) : __builtin_nanf("");
       a.entropy[row] = (float)entropy;
     }
   }
   __syncthreads();
-  const int n = a.segments * a.top;
   for (int i = tid; i < n; i += 256) {
     const u64 key = keys[i];
     if (key == 0) continue;  // of a segment with fewer elements than ranks
@@ -330,19 +343,24 @@ __global__ void __launch_bounds__(256) join_kernel(Args a) {
   }
 }
 
-// A workgroup of 1024 lanes holds 32 elements a lane, 7 (3) of which may belong to the row before; one of 256 a quarter.
+// A lane holds 32 elements; the first 16 bytes of a segment may hold 7 (3) elements in front of it.  Segments are
+// those of a workgroup of 256 lanes, of which a CU runs several (one loads while another sums), unless a row has more
+// than 16 of them.
 struct Plan {
   int threads, segments, segment;
 };
-Plan plan(int rows, int vocab, int type) {
+Plan plan(int vocab, int type) {
   const int spare = type == 2 ? 3 : 7;
   Plan p;
-  p.threads = vocab + spare <= 256 * 32 ? 256 : 1024;
+  p.threads = vocab <= 16 * (256 * 32 - 8) ? 256 : 1024;
   const int most = p.threads * 32 - 8;
-  p.segments = vocab + spare <= p.threads * 32 ? 1 : (vocab + most - 1) / most;
-  p.segment = p.segments == 1 ? vocab : ((vocab + p.segments - 1) / p.segments + 7) / 8 * 8;
-  p.segments = (vocab + p.segment - 1) / p.segment;
-  (void)rows;
+  if (vocab + spare <= p.threads * 32) {
+    p.segments = 1, p.segment = vocab;
+  } else {
+    p.segments = (vocab + most - 1) / most;
+    p.segment = ((vocab + p.segments - 1) / p.segments + 7) / 8 * 8;
+    p.segments = (vocab + p.segment - 1) / p.segment;
+  }
   return p;
 }
 
@@ -363,14 +381,14 @@ int launch(const Args& a, int rows, int threads, hipStream_t s) {
 }
 
 bool sizes_ok(int rows, int vocab, int top, int type) {
-  return rows > 0 && vocab > 0 && vocab <= (1 << 30) && top >= 0 && top <= kMaxTop && top <= vocab && type >= 0 && type <= 2;
+  return rows > 0 && vocab > 0 && vocab <= kMaxVocab && top >= 0 && top <= kMaxTop && top <= vocab && type >= 0 && type <= 2;
 }
 
 }  // namespace
 
 extern "C" size_t serving_token_logprobs_workspace_bytes(int rows, int vocab, int top, int type) {
   if (!sizes_ok(rows, vocab, top, type)) return 0;
-  const Plan p = plan(rows, vocab, type);
+  const Plan p = plan(vocab, type);
   if (p.segments == 1) return 0;
   return (size_t)rows * p.segments * (sizeof(Part) + (size_t)top * sizeof(u64));
 }
@@ -382,7 +400,7 @@ extern "C" int serving_token_logprobs(const void* logits, long long row_stride, 
   if (!sizes_ok(rows, vocab, top, type)) return SERVING_E_SHAPE;
   const int bytes = type == 2 ? 4 : 2;
   if (reinterpret_cast<uintptr_t>(logits) % bytes) return SERVING_E_ALIGN;
-  const Plan p = plan(rows, vocab, type);
+  const Plan p = plan(vocab, type);
   if ((long long)rows * p.segments > 0x7fffffffLL) return SERVING_E_TOO_LARGE;
   const size_t need = serving_token_logprobs_workspace_bytes(rows, vocab, top, type);
   if (need && (!workspace || workspace_bytes < need)) return SERVING_E_WORKSPACE;
