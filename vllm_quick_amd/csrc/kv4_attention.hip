@@ -128,20 +128,24 @@ struct Wave {
 
   __device__ __forceinline__ Wave(const AttendArgs& args) : a(args), c(threadIdx.x & 15), g((threadIdx.x & 63) >> 4) {}
 
-  // The first loads, then the queries while they are under way.
-  __device__ __forceinline__ void begin(const Sequence& s, int b, int kv, int col0, int cols, int first, int last, float* lds) {
+  // Where the keys are, and the loads of the first tile.  No length is asked for: a tile behind the sequence loads what
+  // some block of the table, or block 0, holds, and nobody looks at it.
+  __device__ __forceinline__ void first_loads(int b, int kv, int first, float* lds) {
     kept = lds;
     keeps = false;
     head_base = a.cache + (long long)kv * Kv4<D>::block_bytes(a.block_size);
     block_bytes = Kv4<D>::block_bytes(a.block_size) * a.kv_heads;
     table = scalar(a.tables + b * a.table_stride);
+    last_page = a.table_width - 1;
+    aim(first, block_of(2 * first), block_of(2 * first + 1));
+    load_keys();
+    load_params();
+    load_values();
+  }
+
+  // The queries.
+  __device__ __forceinline__ void begin(const Sequence& s, int kv, int col0, int cols) {
     last_page = max(0, page_of((s.length - 1) >> 4));
-    if (first < last) {
-      aim(first, block_of(2 * first), block_of(2 * first + 1));
-      load_keys();
-      load_params();
-      load_values();
-    }
     vref = 0x1p-40f;
     weight_log = kWeightLog + 40.f;
     float x[NC][kSteps][8], big = 0.f;
@@ -373,7 +377,7 @@ struct Wave {
     load_values();
   }
 
-  // Runs over tiles first, first + stride, .. < last, the first of them loaded by begin(); all columns see all of the tiles that lie in whole_from ..
+  // Runs over tiles first, first + stride, .. < last, the first of them loaded; all columns see all of the tiles that lie in whole_from ..
   // whole_to - 1 of the keys.
   __device__ __forceinline__ void run(int first, int last, int stride, int length, int whole_from, int whole_to) {
     if (first >= last) return;
@@ -482,6 +486,11 @@ __global__ void __launch_bounds__(64 * WAVES, NC == 1 ? 3 : 2) attend_split_kern
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int pair = blockIdx.x, b = pair / a.kv_heads, kv = pair - b * a.kv_heads;
   const int split = blockIdx.y, tile = blockIdx.z;
+  const int per_piece = a.chunk / kTile;
+  Wave<T, D, NC> w(a);
+  // Without a window a piece begins where it does whatever the length, which is under way meanwhile: one round trip to
+  // memory less before the first keys.
+  if (a.window == 0) w.first_loads(b, kv, split * per_piece + wave, &part[wave][0][0]);
   const Sequence s = sequence(a, b);
   const int queries = min(s.queries, a.max_query_len), cols = queries * a.group;
   if (tile == 0 && split == 0 && queries < s.queries) refuse_rows<T, D>(a, s, kv);
@@ -490,11 +499,10 @@ __global__ void __launch_bounds__(64 * WAVES, NC == 1 ? 3 : 2) attend_split_kern
   const Range r = range(a, s, col0, min(cols - 1, col0 + kCols - 1));
   const int pieces = pieces_of(a, r);
   if (split >= pieces) return;
-  const int per_piece = a.chunk / kTile;
   const int t0 = r.first_tile + split * per_piece + wave;
   const int t1 = split == pieces - 1 ? r.last_tile : r.first_tile + (split + 1) * per_piece;
-  Wave<T, D, NC> w(a);
-  w.begin(s, b, kv, col0, cols, t0, t1, &part[wave][0][0]);
+  if (a.window > 0) w.first_loads(b, kv, t0, &part[wave][0][0]);
+  w.begin(s, kv, col0, cols);
   w.run(t0, t1, WAVES, s.length, r.whole_from, r.whole_to);
 
   w.set_aside();
@@ -630,7 +638,8 @@ __global__ void __launch_bounds__(256, 2) attend_prompt_kernel(AttendArgs a) {
   if (col0 >= cols) return;
   const Range r = range(a, s, col0, min(cols - 1, col0 + kCols - 1));
   Wave<T, D, NC> w(a);
-  w.begin(s, b, kv, col0, cols, r.first_tile, r.last_tile, &part[wave][0][0]);
+  w.first_loads(b, kv, r.first_tile, &part[wave][0][0]);
+  w.begin(s, kv, col0, cols);
   w.run(r.first_tile, r.last_tile, 1, s.length, r.whole_from, r.whole_to);
   if (w.keeps) w.set_aside();
 #pragma unroll

@@ -38,9 +38,11 @@ void raise_for(int rc, const char* what) {
   }
 }
 
-void need(bool ok, const char* what, const std::string& why) {
-  if (!ok) throw std::invalid_argument(std::string(what) + ": " + why);
-}
+// The message is put together only where it is needed.
+#define NEED(ok, ...)                                                          \
+  do {                                                                         \
+    if (!(ok)) throw std::invalid_argument(c10::str(what, ": ", __VA_ARGS__)); \
+  } while (0)
 
 std::string shape_of(const Tensor& t) {
   std::string s = "[";
@@ -82,13 +84,11 @@ Tensor ints(const Tensor& t) { return t.is_contiguous() ? t : t.contiguous(); }
 // D and P of a cache [blocks, kv heads, P (D + 8)] for heads of head_size elements.
 int64_t block_size_of(const Tensor& cache, int64_t head_size, const char* what) {
   typed(cache, at::kByte, what, "cache");
-  need(head_size == 64 || head_size == 128, what, "head_size must be 64 or 128, got " + std::to_string(head_size));
-  need(cache.dim() == 3 && cache.size(0) > 0 && cache.size(1) > 0 && cache.size(2) > 0 && cache.size(2) % (head_size + 8) == 0 &&
-           (cache.size(2) / (head_size + 8)) % 16 == 0,
-       what, "cache must be [blocks, kv heads, block_size * (head_size + 8)] with a block_size that is a multiple of 16, got " +
-                 shape_of(cache) + " for heads of " + std::to_string(head_size));
-  need(cache.is_contiguous(), what, "cache must be contiguous");
-  need(cache.size(0) <= kMostInt && cache.size(1) <= 65535 && cache.size(2) / (head_size + 8) <= 4096, what, "cache is too large");
+  NEED(head_size == 64 || head_size == 128, "head_size must be 64 or 128, got ", head_size);
+  NEED(cache.dim() == 3 && cache.size(0) > 0 && cache.size(1) > 0 && cache.size(2) > 0 && cache.size(2) % (head_size + 8) == 0 &&
+           (cache.size(2) / (head_size + 8)) % 16 == 0, "cache must be [blocks, kv heads, block_size * (head_size + 8)] with a block_size that is a multiple of 16, got ", shape_of(cache), " for heads of ", head_size);
+  NEED(cache.is_contiguous(), "cache must be contiguous");
+  NEED(cache.size(0) <= kMostInt && cache.size(1) <= 65535 && cache.size(2) / (head_size + 8) <= 4096, "cache is too large");
   TORCH_CHECK(reinterpret_cast<uintptr_t>(cache.data_ptr()) % 16 == 0, what, ": cache is not 16-byte aligned");
   return cache.size(2) / (head_size + 8);
 }
@@ -102,20 +102,17 @@ Tensor rope_append_kv4(const Tensor& positions, const Tensor& query, const Tenso
   typed(cos_sin, at::kFloat, what, "cos_sin");
   typed(positions, at::kLong, what, "positions");
   typed(slots, at::kLong, what, "slots");
-  need(query.dim() == 3, what, "query must be [tokens, heads, head_size], got " + shape_of(query));
+  NEED(query.dim() == 3, "query must be [tokens, heads, head_size], got ", shape_of(query));
   const int64_t tokens = query.size(0), heads = query.size(1), d = query.size(2);
   const int64_t block_size = block_size_of(cache, d, what), kv = cache.size(1);
   for (const auto& [t, name] : {std::pair<const Tensor&, const char*>(key, "key"), {value, "value"}})
-    need(t.dim() == 3 && t.size(0) == tokens && t.size(1) == kv && t.size(2) == d, what,
-         std::string(name) + " must be [" + std::to_string(tokens) + ", " + std::to_string(kv) + ", " + std::to_string(d) +
-             "] as query and cache have it, got " + shape_of(t));
-  need(positions.dim() == 1 && positions.size(0) == tokens, what, "positions must be [tokens], got " + shape_of(positions));
-  need(slots.dim() == 1 && slots.size(0) == tokens, what, "slots must be [tokens], got " + shape_of(slots));
-  need(cos_sin.dim() == 2, what, "cos_sin must be [positions, rotary], got " + shape_of(cos_sin));
+    NEED(t.dim() == 3 && t.size(0) == tokens && t.size(1) == kv && t.size(2) == d, name, " must be [", tokens, ", ", kv, ", ", d, "] as query and cache have it, got ", shape_of(t));
+  NEED(positions.dim() == 1 && positions.size(0) == tokens, "positions must be [tokens], got ", shape_of(positions));
+  NEED(slots.dim() == 1 && slots.size(0) == tokens, "slots must be [tokens], got ", shape_of(slots));
+  NEED(cos_sin.dim() == 2, "cos_sin must be [positions, rotary], got ", shape_of(cos_sin));
   const int64_t rotary = cos_sin.size(1);
-  need(rotary % 16 == 0 && rotary <= d, what,
-       "the rotated part of a head must be a multiple of 16 elements and no larger than a head, got " + std::to_string(rotary));
-  need(tokens <= (1 << 30) && heads <= 65535, what, "too many tokens or heads");
+  NEED(rotary % 16 == 0 && rotary <= d, "the rotated part of a head must be a multiple of 16 elements and no larger than a head, got ", rotary);
+  NEED(tokens <= (1 << 30) && heads <= 65535, "too many tokens or heads");
   for (const auto& [t, name] : {std::pair<const Tensor&, const char*>(query, "query"), {key, "key"}, {value, "value"},
                                 {cos_sin, "cos_sin"}, {cache, "cache"}, {positions, "positions"}, {slots, "slots"}}) {
     on_gpu(t, query, what, name);
@@ -143,7 +140,7 @@ std::tuple<Tensor, Tensor> kv4_read(const Tensor& cache, const Tensor& slots, in
   TORCH_CHECK(dtype == at::kHalf || dtype == at::kBFloat16, what, ": dtype must be Half or BFloat16, got ", dtype);
   const int64_t block_size = block_size_of(cache, head_size, what);
   typed(slots, at::kLong, what, "slots");
-  need(slots.dim() == 1, what, "slots must be [rows], got " + shape_of(slots));
+  NEED(slots.dim() == 1, "slots must be [rows], got ", shape_of(slots));
   on_gpu(cache, cache, what, "cache");
   on_gpu(slots, cache, what, "slots");
   const OptionalHIPGuardMasqueradingAsCUDA guard(cache.device());
@@ -165,29 +162,25 @@ Tensor paged_attention_kv4(const Tensor& query, const Tensor& cache, const Tenso
   const bool bf16 = activations(query, what, "query");
   typed(block_tables, at::kInt, what, "block_tables");
   typed(seq_lens, at::kInt, what, "seq_lens");
-  need(query.dim() == 3, what, "query must be [tokens, heads, head_size], got " + shape_of(query));
+  NEED(query.dim() == 3, "query must be [tokens, heads, head_size], got ", shape_of(query));
   const int64_t tokens = query.size(0), heads = query.size(1), d = query.size(2);
   const int64_t block_size = block_size_of(cache, d, what), kv = cache.size(1);
-  need(heads > 0 && heads <= 65535 && heads % kv == 0, what,
-       "query has " + std::to_string(heads) + " heads, which the cache's " + std::to_string(kv) + " cannot share");
-  need(seq_lens.dim() == 1, what, "seq_lens must be [sequences], got " + shape_of(seq_lens));
+  NEED(heads > 0 && heads <= 65535 && heads % kv == 0, "query has ", heads, " heads, which the cache's ", kv, " cannot share");
+  NEED(seq_lens.dim() == 1, "seq_lens must be [sequences], got ", shape_of(seq_lens));
   const int64_t seqs = seq_lens.size(0);
-  need(block_tables.dim() == 2 && block_tables.size(0) == seqs, what,
-       "block_tables must be [sequences, blocks], got " + shape_of(block_tables));
-  need(max_seq_len > 0 && max_seq_len <= (1 << 27) && block_tables.size(1) * block_size <= (1 << 27), what,
-       "sequences are of 1 to 2^27 tokens");
-  need(window >= 0 && window <= kMostInt, what, "window must not be negative");
-  need(max_query_len > 0 && max_query_len <= kMostInt, what, "max_query_len must be positive");
-  need(std::isfinite(scale) && std::isfinite((float)scale), what, "scale must be finite");
-  need(tokens <= kMostInt, what, "too many tokens");
+  NEED(block_tables.dim() == 2 && block_tables.size(0) == seqs, "block_tables must be [sequences, blocks], got ", shape_of(block_tables));
+  NEED(max_seq_len > 0 && max_seq_len <= (1 << 27) && block_tables.size(1) * block_size <= (1 << 27), "sequences are of 1 to 2^27 tokens");
+  NEED(window >= 0 && window <= kMostInt, "window must not be negative");
+  NEED(max_query_len > 0 && max_query_len <= kMostInt, "max_query_len must be positive");
+  NEED(std::isfinite(scale) && std::isfinite((float)scale), "scale must be finite");
+  NEED(tokens <= kMostInt, "too many tokens");
   if (query_start) {
     typed(*query_start, at::kInt, what, "query_start");
-    need(query_start->dim() == 1 && query_start->size(0) == seqs + 1, what,
-         "query_start must be [sequences + 1], got " + shape_of(*query_start));
+    NEED(query_start->dim() == 1 && query_start->size(0) == seqs + 1, "query_start must be [sequences + 1], got ", shape_of(*query_start));
     on_gpu(*query_start, query, what, "query_start");
   } else {
-    need(tokens == seqs, what, "without query_start there is one query for each sequence");
-    need(max_query_len == 1, what, "without query_start max_query_len is 1");
+    NEED(tokens == seqs, "without query_start there is one query for each sequence");
+    NEED(max_query_len == 1, "without query_start max_query_len is 1");
   }
   for (const auto& [t, name] : {std::pair<const Tensor&, const char*>(query, "query"), {cache, "cache"},
                                 {block_tables, "block_tables"}, {seq_lens, "seq_lens"}})
@@ -197,15 +190,14 @@ Tensor paged_attention_kv4(const Tensor& query, const Tensor& cache, const Tenso
     typed(*out_, query.scalar_type(), what, "out");
     on_gpu(*out_, query, what, "out");
     no_gradient(*out_, what, "out");
-    need(out_->sizes() == query.sizes() && out_->is_contiguous(), what,
-         "out must be a contiguous " + shape_of(query) + ", got " + shape_of(*out_));
+    NEED(out_->sizes() == query.sizes() && out_->is_contiguous(), "out must be a contiguous ", shape_of(query), ", got ", shape_of(*out_));
     TORCH_CHECK(reinterpret_cast<uintptr_t>(out_->data_ptr()) % 16 == 0, what, ": out is not 16-byte aligned");
   }
   const OptionalHIPGuardMasqueradingAsCUDA guard(query.device());
   Tensor out = out_ ? *out_ : torch::empty({tokens, heads, d}, query.options());
   if (tokens == 0 || seqs == 0) return out;
   if (block_tables.size(1) == 0) {  // no sequence has a block: every row sees nothing
-    need(!query_start, what, "block_tables has no columns");
+    NEED(!query_start, "block_tables has no columns");
     return out.zero_();
   }
   const Tensor q = heads_of(query), lens = ints(seq_lens);
@@ -230,12 +222,11 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> token_logprobs(const Tensor& logits, 
   TORCH_CHECK(type == at::kHalf || type == at::kBFloat16 || type == at::kFloat, what,
               ": expected scalar type Half, BFloat16 or Float but found ", type, " for logits");
   typed(token_ids, at::kLong, what, "token_ids");
-  need(logits.dim() == 2 && logits.size(1) > 0, what, "logits must be [rows, vocabulary], got " + shape_of(logits));
+  NEED(logits.dim() == 2 && logits.size(1) > 0, "logits must be [rows, vocabulary], got ", shape_of(logits));
   const int64_t rows = logits.size(0), vocab = logits.size(1);
-  need(token_ids.dim() == 1 && token_ids.size(0) == rows, what, "token_ids must be [rows], got " + shape_of(token_ids));
-  need(top_n >= 0 && top_n <= 64 && top_n <= vocab, what,
-       "top_n must be from 0 to 64 and no more than the vocabulary, got " + std::to_string(top_n));
-  need(rows <= kMostInt && vocab <= 64 * 32760, what, "a vocabulary has at most 2096640 tokens, and there are too many rows or tokens here");
+  NEED(token_ids.dim() == 1 && token_ids.size(0) == rows, "token_ids must be [rows], got ", shape_of(token_ids));
+  NEED(top_n >= 0 && top_n <= 64 && top_n <= vocab, "top_n must be from 0 to 64 and no more than the vocabulary, got ", top_n);
+  NEED(rows <= kMostInt && vocab <= 64 * 32760, "a vocabulary has at most 2096640 tokens, and there are too many rows or tokens here");
   on_gpu(logits, logits, what, "logits");
   on_gpu(token_ids, logits, what, "token_ids");
   no_gradient(logits, what, "logits");

@@ -18,6 +18,7 @@ using namespace serving;
 constexpr int kMaxTop = 64;       // groups that are ranked for the bound
 constexpr int kCandidates = 1024;  // elements not below the bound that LDS takes; more (rows of equals) go the long way
 
+constexpr int kFewRows = 256;  // a workgroup of 1024 lanes for each CU
 constexpr int kMaxVocab = 64 * 32760;  // 64 segments: a lane of the join each, and their keys in LDS
 
 typedef unsigned long long u64;
@@ -64,6 +65,14 @@ __device__ __forceinline__ int index_of(u64 key) { return (int)(0xffffffffu - (u
 
 __device__ __forceinline__ float larger(float a, float b) { return __builtin_elementwise_maximum(a, b); }  // NaN if one is
 
+// What a pass made of the elements is made anew by the next one: 32 differences kept from pass to pass would take the
+// registers of another workgroup.
+template <int NV>
+__device__ __forceinline__ void forget(u32x4 (&v)[NV]) {
+#pragma unroll
+  for (int k = 0; k < NV; ++k) asm("" : "+v"(v[k]));
+}
+
 template <typename V, typename F>
 __device__ __forceinline__ V wave_all(V v, F f) {
 #pragma unroll
@@ -90,7 +99,7 @@ struct Args {
 };
 
 template <int TYPE, int THREADS, int NV>
-__global__ void __launch_bounds__(THREADS, 4) logprobs_kernel(Args a) {
+__global__ void __launch_bounds__(THREADS, THREADS == 256 ? 6 : 4) logprobs_kernel(Args a) {
   typedef Logits<TYPE> X;
   constexpr int kWaves = THREADS / 64;
   constexpr float kLog2e = 1.44269504088896340736f;
@@ -111,23 +120,22 @@ __global__ void __launch_bounds__(THREADS, 4) logprobs_kernel(Args a) {
   const u32x4* words = reinterpret_cast<const u32x4*>(base - skip * X::kBytes);
   if (tid == 0) n_candidates = 0;
 
+  const auto fetch = [&](int k) {
+    const int e = (k * THREADS + tid) * X::kEach - skip;  // of this lane's first element in the segment
+    u32x4 w = {0u, 0u, 0u, 0u};
+    // (16 aligned bytes that hold one of the row's elements: never outside the pages of its tensor)
+    const bool some = e < size && e > -X::kEach;
+    if (some) w = words[k * THREADS + tid];
+    if (!some || e < 0 || e + X::kEach > size) {
+#pragma unroll
+      for (int i = 0; i < X::kEach; ++i)
+        if (e + i < 0 || e + i >= size) X::hide(w, i);
+    }
+    return w;
+  };
   u32x4 v[NV];
 #pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    const int e = (k * THREADS + tid) * X::kEach - skip;  // of this lane's first element in the segment
-    // (16 aligned bytes that hold one of the row's elements: never outside the pages of its tensor)
-    if (e < size && e > -X::kEach) {
-      v[k] = words[k * THREADS + tid];
-      if (e < 0 || e + X::kEach > size) {
-#pragma unroll
-        for (int i = 0; i < X::kEach; ++i)
-          if (e + i < 0 || e + i >= size) X::hide(v[k], i);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < X::kEach; ++i) X::hide(v[k], i);
-    }
-  }
+  for (int k = 0; k < NV; ++k) v[k] = fetch(k);
   float given = 0.f;
   long long token = -1;
   if (a.segments == 1 && tid == 0) {
@@ -146,6 +154,7 @@ __global__ void __launch_bounds__(THREADS, 4) logprobs_kernel(Args a) {
 #pragma unroll
     for (int i = 0; i < X::kEach; ++i) mine = larger(mine, X::get(v[k], i));
   lane_most[wave][lane] = ordered(mine);
+  forget(v);
   __syncthreads();
   // the 64 groups: the elements of equal lanes of all waves
   uint32_t group = 0;
@@ -159,11 +168,13 @@ __global__ void __launch_bounds__(THREADS, 4) logprobs_kernel(Args a) {
   for (int k = 0; k < NV; ++k)
 #pragma unroll
     for (int i = 0; i < X::kEach; ++i) {
-      const float d = fmaxf(X::get(v[k], i) - most, -10000.f);  // (-inf adds nothing, and not 0 * inf)
-      const float p = __builtin_amdgcn_exp2f(d * kLog2e);
+      const float d = fmaxf(X::get(v[k], i) - most, -10000.f) * kLog2e;  // (-inf adds nothing, and not 0 * inf)
+      const float p = __builtin_amdgcn_exp2f(d);
       rest += p;
       weighted = __builtin_fmaf(p, d, weighted);
     }
+  weighted *= 0.69314718055994530942f;
+  forget(v);
   if (mine == most) {  // the few lanes that hold a maximum sum again without it
     rest = 0.f;
     for (int k = 0; k < NV; ++k)
@@ -191,20 +202,23 @@ __global__ void __launch_bounds__(THREADS, 4) logprobs_kernel(Args a) {
     if (ahead == (uint32_t)a.top - 1) shared_bound = group & ~63u;
   }
   __syncthreads();
+  forget(v);
   if (a.top > 0) {
     const uint32_t bound = shared_bound;
     const float border = bound < ordered(-__builtin_inff()) ? -__builtin_inff() : unordered(bound);
     if (most != most) {  // a row with a NaN: ordered numbers know where it stands, comparisons do not
-#pragma unroll
-      for (int k = 0; k < NV; ++k)
+#pragma unroll 1
+      for (int k = 0; k < NV; ++k) {
+        const u32x4 w = fetch(k);
         for (int i = 0; i < X::kEach; ++i) {
-          const float x = X::get(v[k], i);
+          const float x = X::get(w, i);
           const int e = (k * THREADS + tid) * X::kEach - skip + i;
           if (ordered(x) >= bound && e >= 0 && e < size) {
             const int at = atomicAdd(&n_candidates, 1);
             if (at < kCandidates) candidates[at] = key_of(x, begin + e);
           }
         }
+      }
     } else if (mine >= border) {
 #pragma unroll
       for (int k = 0; k < NV; ++k)
@@ -266,12 +280,13 @@ __global__ void __launch_bounds__(THREADS, 4) logprobs_kernel(Args a) {
   u64 last = ~0ull;
   for (int r = 0; r < want; ++r) {
     u64 best = 0;
-#pragma unroll
+#pragma unroll 1
     for (int k = 0; k < NV; ++k) {
+      const u32x4 w = fetch(k);
       const int e = (k * THREADS + tid) * X::kEach - skip;
 #pragma unroll
       for (int i = 0; i < X::kEach; ++i) {
-        const u64 key = key_of(X::get(v[k], i), begin + e + i);
+        const u64 key = key_of(X::get(w, i), begin + e + i);
         if (e + i >= 0 && e + i < size && key < last && key > best) best = key;
       }
     }
@@ -287,20 +302,23 @@ __global__ void __launch_bounds__(THREADS, 4) logprobs_kernel(Args a) {
 }
 
 // Joins the segments of a row: sums by one wave, a lane a segment, the most likely tokens by counting the keys ahead
-// of each.
-constexpr int kJoinKeys = 4096;
-
-template <int TYPE>
-__global__ void __launch_bounds__(256) join_kernel(Args a) {
+// of each.  Four rows a workgroup, a wave each, where there are many rows with few keys (4096 rows of 80 keys 10 us
+// against 18; 64 of them 7 against 4.5).
+template <int TYPE, int ROWS>
+__global__ void __launch_bounds__(256) join_kernel(Args a, int rows) {
   typedef Logits<TYPE> X;
-  __shared__ double shared_log_z;
-  __shared__ float shared_most;
-  __shared__ u64 keys[kJoinKeys];
-  const int row = blockIdx.x, tid = threadIdx.x;
+  constexpr int kLanes = 256 / ROWS, kKeys = ROWS == 1 ? 4096 : 128;
+  __shared__ double shared_log_z[ROWS];
+  __shared__ float shared_most[ROWS];
+  __shared__ u64 all_keys[ROWS][kKeys];
+  const int which = threadIdx.x / kLanes, tid = threadIdx.x % kLanes;
+  const int row = blockIdx.x * ROWS + which;
+  const bool on = row < rows;
   const Part* parts = a.parts + (long long)row * a.segments;
-  const int n = a.segments * a.top;
-  for (int i = tid; i < n; i += 256) keys[i] = a.keys[(long long)row * n + i];
-  if (tid < 64) {
+  const int n = on ? a.segments * a.top : 0;
+  u64* keys = all_keys[which];
+  for (int i = tid; i < n; i += kLanes) keys[i] = a.keys[(long long)row * n + i];
+  if (on && tid < 64) {
     const long long token = a.token_ids[row];
     const bool known = token >= 0 && token < a.vocab;
     const uint8_t* p = a.logits + row * a.row_stride + (known ? token : 0) * X::kBytes;
@@ -323,14 +341,14 @@ __global__ void __launch_bounds__(256) join_kernel(Args a) {
     double log_z = __builtin_nan(""), entropy = __builtin_nan("");
     if (__builtin_isfinite(most)) finish(count, rest, weighted, log_z, entropy);
     if (tid == 0) {
-      shared_log_z = log_z;
-      shared_most = most;
+      shared_log_z[which] = log_z;
+      shared_most[which] = most;
       a.logprob[row] = known ? (float)((double)(x - most) - log_z) : __builtin_nanf("");
       a.entropy[row] = (float)entropy;
     }
   }
   __syncthreads();
-  for (int i = tid; i < n; i += 256) {
+  for (int i = tid; i < n; i += kLanes) {
     const u64 key = keys[i];
     if (key == 0) continue;  // of a segment with fewer elements than ranks
     int ahead = 0;
@@ -338,21 +356,22 @@ __global__ void __launch_bounds__(256) join_kernel(Args a) {
     if (ahead < a.top) {
       a.top_ids[(long long)row * a.top + ahead] = index_of(key);
       a.top_logprobs[(long long)row * a.top + ahead] =
-          (float)((double)(unordered((uint32_t)(key >> 32)) - shared_most) - shared_log_z);
+          (float)((double)(unordered((uint32_t)(key >> 32)) - shared_most[which]) - shared_log_z[which]);
     }
   }
 }
 
-// A lane holds 32 elements; the first 16 bytes of a segment may hold 7 (3) elements in front of it.  Segments are
-// those of a workgroup of 256 lanes, of which a CU runs several (one loads while another sums), unless a row has more
-// than 16 of them.
+// A lane holds 32 elements; the first 16 bytes of a segment may hold 7 (3) elements in front of it.  A workgroup of
+// 1024 lanes takes a row of up to 32760 tokens alone, which is one launch instead of two; where there are enough rows to
+// fill the chip, segments of 256 lanes do more, since a CU runs several (one loads while another sums): 4096 x 32000 fp32
+// 116 us against 222.
 struct Plan {
   int threads, segments, segment;
 };
-Plan plan(int vocab, int type) {
+Plan plan(int rows, int vocab, int type) {
   const int spare = type == 2 ? 3 : 7;
   Plan p;
-  p.threads = vocab <= 16 * (256 * 32 - 8) ? 256 : 1024;
+  p.threads = vocab > 16 * (256 * 32 - 8) || (vocab + spare > 256 * 32 && vocab + spare <= 1024 * 32 && rows <= kFewRows) ? 1024 : 256;
   const int most = p.threads * 32 - 8;
   if (vocab + spare <= p.threads * 32) {
     p.segments = 1, p.segment = vocab;
@@ -375,7 +394,10 @@ int launch(const Args& a, int rows, int threads, hipStream_t s) {
   if (a.segments > 1) {
     const int rc = serving_after_launch();
     if (rc != SERVING_OK) return rc;
-    hipLaunchKernelGGL((join_kernel<TYPE>), dim3((unsigned)rows), dim3(256), 0, s, a);
+    if (a.segments * a.top <= 128 && rows >= 1024)
+      hipLaunchKernelGGL((join_kernel<TYPE, 4>), dim3((unsigned)((rows + 3LL) / 4)), dim3(256), 0, s, a, rows);
+    else
+      hipLaunchKernelGGL((join_kernel<TYPE, 1>), dim3((unsigned)rows), dim3(256), 0, s, a, rows);
   }
   return serving_after_launch();
 }
@@ -388,7 +410,7 @@ bool sizes_ok(int rows, int vocab, int top, int type) {
 
 extern "C" size_t serving_token_logprobs_workspace_bytes(int rows, int vocab, int top, int type) {
   if (!sizes_ok(rows, vocab, top, type)) return 0;
-  const Plan p = plan(vocab, type);
+  const Plan p = plan(rows, vocab, type);
   if (p.segments == 1) return 0;
   return (size_t)rows * p.segments * (sizeof(Part) + (size_t)top * sizeof(u64));
 }
@@ -400,7 +422,7 @@ extern "C" int serving_token_logprobs(const void* logits, long long row_stride, 
   if (!sizes_ok(rows, vocab, top, type)) return SERVING_E_SHAPE;
   const int bytes = type == 2 ? 4 : 2;
   if (reinterpret_cast<uintptr_t>(logits) % bytes) return SERVING_E_ALIGN;
-  const Plan p = plan(vocab, type);
+  const Plan p = plan(rows, vocab, type);
   if ((long long)rows * p.segments > 0x7fffffffLL) return SERVING_E_TOO_LARGE;
   const size_t need = serving_token_logprobs_workspace_bytes(rows, vocab, top, type);
   if (need && (!workspace || workspace_bytes < need)) return SERVING_E_WORKSPACE;
