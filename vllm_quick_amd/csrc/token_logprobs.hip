@@ -11,6 +11,8 @@
 // ahead of it.  Equal elements are told apart by their index, which makes the order total and the result one of its own.
 #include "kv4_cache.h"
 
+#include <type_traits>
+
 namespace {
 
 using namespace serving;
@@ -65,14 +67,6 @@ __device__ __forceinline__ int index_of(u64 key) { return (int)(0xffffffffu - (u
 
 __device__ __forceinline__ float larger(float a, float b) { return __builtin_elementwise_maximum(a, b); }  // NaN if one is
 
-// What a pass made of the elements is made anew by the next one: 32 differences kept from pass to pass would take the
-// registers of another workgroup.
-template <int NV>
-__device__ __forceinline__ void forget(u32x4 (&v)[NV]) {
-#pragma unroll
-  for (int k = 0; k < NV; ++k) asm("" : "+v"(v[k]));
-}
-
 template <typename V, typename F>
 __device__ __forceinline__ V wave_all(V v, F f) {
 #pragma unroll
@@ -99,7 +93,7 @@ struct Args {
 };
 
 template <int TYPE, int THREADS, int NV>
-__global__ void __launch_bounds__(THREADS, THREADS == 256 ? 6 : 4) logprobs_kernel(Args a) {
+__global__ void __launch_bounds__(THREADS, 4) logprobs_kernel(Args a) {
   typedef Logits<TYPE> X;
   constexpr int kWaves = THREADS / 64;
   constexpr float kLog2e = 1.44269504088896340736f;
@@ -109,7 +103,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 6 : 4) logprobs_kern
   __shared__ u64 candidates[kCandidates];
   __shared__ u64 wave_best[kWaves];
   __shared__ int n_candidates;
-  __shared__ uint32_t shared_bound;
+  __shared__ int groups_ahead[64];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int row = blockIdx.x / a.segments, seg = blockIdx.x - row * a.segments;
   const int begin = seg * a.segment;                         // of this segment in its row
@@ -119,6 +113,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 6 : 4) logprobs_kern
   const int skip = (int)((reinterpret_cast<uintptr_t>(base) & 15u) / X::kBytes);  // of the first 16 bytes, not ours
   const u32x4* words = reinterpret_cast<const u32x4*>(base - skip * X::kBytes);
   if (tid == 0) n_candidates = 0;
+  if (tid < 64) groups_ahead[tid] = 0;
 
   const auto fetch = [&](int k) {
     const int e = (k * THREADS + tid) * X::kEach - skip;  // of this lane's first element in the segment
@@ -154,7 +149,6 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 6 : 4) logprobs_kern
 #pragma unroll
     for (int i = 0; i < X::kEach; ++i) mine = larger(mine, X::get(v[k], i));
   lane_most[wave][lane] = ordered(mine);
-  forget(v);
   __syncthreads();
   // the 64 groups: the elements of equal lanes of all waves
   uint32_t group = 0;
@@ -164,47 +158,49 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 6 : 4) logprobs_kern
 
   float rest = 0.f, weighted = 0.f;
   int count = 0;
+  const auto sum = [&](auto with_maximum) {
 #pragma unroll
-  for (int k = 0; k < NV; ++k)
-#pragma unroll
-    for (int i = 0; i < X::kEach; ++i) {
-      const float d = fmaxf(X::get(v[k], i) - most, -10000.f) * kLog2e;  // (-inf adds nothing, and not 0 * inf)
-      const float p = __builtin_amdgcn_exp2f(d);
-      rest += p;
-      weighted = __builtin_fmaf(p, d, weighted);
-    }
-  weighted *= 0.69314718055994530942f;
-  forget(v);
-  if (mine == most) {  // the few lanes that hold a maximum sum again without it
-    rest = 0.f;
-    for (int k = 0; k < NV; ++k)
+    for (int k = 0; k < NV; ++k) {
 #pragma unroll
       for (int i = 0; i < X::kEach; ++i) {
-        const float d = fmaxf(X::get(v[k], i) - most, -10000.f);
-        if (d == 0.f)
-          ++count;
-        else
-          rest += __builtin_amdgcn_exp2f(d * kLog2e);
+        const float d = fmaxf(X::get(v[k], i) - most, -10000.f) * kLog2e;  // (-inf adds nothing, and not 0 * inf)
+        const float p = __builtin_amdgcn_exp2f(d);
+        if (with_maximum) {
+          count += d == 0.f;
+          rest += d == 0.f ? 0.f : p;
+        } else {
+          rest += p;
+        }
+        weighted = __builtin_fmaf(p, d, weighted);
       }
+      __builtin_amdgcn_sched_barrier(0);  // (16 bytes at a time: more at once would only take registers)
+    }
+  };
+  if (__any(mine == most)) {  // the wave or two that hold a maximum
+    asm volatile("");  // (keeps this a branch)
+    sum(std::true_type());
+  } else {
+    sum(std::false_type());
   }
+  weighted *= 0.69314718055994530942f;
   rest = wave_all(rest, [](float p, float q) { return p + q; });
   weighted = wave_all(weighted, [](float p, float q) { return p + q; });
   count = wave_all(count, [](int p, int q) { return p + q; });
   if (lane == 0) sums[wave][0] = rest, sums[wave][1] = weighted, counts[wave] = count;
 
-  // the n-th largest group maximum: each lane of the last wave counts the groups ahead of its own (told apart by the
-  // lane in the last six bits; what these held only lowers the bound)
-  if (a.top > 0 && wave == kWaves - 1) {
-    const uint32_t own = (group & ~63u) | (uint32_t)(63 - lane);
-    uint32_t ahead = 0;
+  // The n-th largest group maximum: each lane counts the groups ahead of its own, a share of them in each wave (told
+  // apart by the lane in the last six bits; what these held only lowers the bound).
+  const uint32_t own = (group & ~63u) | (uint32_t)(63 - lane);
+  if (a.top > 0) {
+    int ahead = 0;
 #pragma unroll
-    for (int g = 0; g < 64; ++g) ahead += (uint32_t)__builtin_amdgcn_readlane(own, g) > own ? 1u : 0u;
-    if (ahead == (uint32_t)a.top - 1) shared_bound = group & ~63u;
+    for (int i = 0; i < 64 / kWaves; ++i)
+      ahead += (uint32_t)__builtin_amdgcn_readlane(own, __builtin_amdgcn_readfirstlane(wave) * (64 / kWaves) + i) > own;
+    atomicAdd(&groups_ahead[lane], ahead);
   }
   __syncthreads();
-  forget(v);
   if (a.top > 0) {
-    const uint32_t bound = shared_bound;
+    const uint32_t bound = __builtin_amdgcn_readlane(own, __builtin_ctzll(__ballot(groups_ahead[lane] == a.top - 1))) & ~63u;
     const float border = bound < ordered(-__builtin_inff()) ? -__builtin_inff() : unordered(bound);
     if (most != most) {  // a row with a NaN: ordered numbers know where it stands, comparisons do not
 #pragma unroll 1
@@ -221,18 +217,21 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 6 : 4) logprobs_kern
       }
     } else if (mine >= border) {
 #pragma unroll
-      for (int k = 0; k < NV; ++k)
+      for (int k = 0; k < NV; ++k) {
+        bool some = false;
+#pragma unroll
+        for (int i = 0; i < X::kEach; ++i) some |= X::get(v[k], i) >= border;
+        if (!some) continue;
+        const int e = (k * THREADS + tid) * X::kEach - skip;
 #pragma unroll
         for (int i = 0; i < X::kEach; ++i) {
           const float x = X::get(v[k], i);
-          if (x >= border) {
-            const int e = (k * THREADS + tid) * X::kEach - skip + i;
-            if (e >= 0 && e < size) {
-              const int at = atomicAdd(&n_candidates, 1);
-              if (at < kCandidates) candidates[at] = key_of(x, begin + e);
-            }
+          if (x >= border && e + i >= 0 && e + i < size) {
+            const int at = atomicAdd(&n_candidates, 1);
+            if (at < kCandidates) candidates[at] = key_of(x, begin + e + i);
           }
         }
+      }
     }
   }
   __syncthreads();
@@ -271,6 +270,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 6 : 4) logprobs_kern
     for (int i = tid; i < n; i += THREADS) {
       const u64 key = candidates[i];
       int ahead = 0;
+#pragma unroll 8
       for (int j = 0; j < n; ++j) ahead += candidates[j] > key;
       if (ahead < want) place(ahead, key);
     }
@@ -307,16 +307,18 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 6 : 4) logprobs_kern
 template <int TYPE, int ROWS>
 __global__ void __launch_bounds__(256) join_kernel(Args a, int rows) {
   typedef Logits<TYPE> X;
-  constexpr int kLanes = 256 / ROWS, kKeys = ROWS == 1 ? 4096 : 128;
+  constexpr int kLanes = 256 / ROWS, kKeys = ROWS == 1 ? 4096 : 128, kRanked = ROWS == 1 ? 512 : 128;
   __shared__ double shared_log_z[ROWS];
   __shared__ float shared_most[ROWS];
-  __shared__ u64 all_keys[ROWS][kKeys];
+  __shared__ u64 all_keys[ROWS][kKeys], ranked[ROWS][kRanked], bound[ROWS];
+  __shared__ int n_ranked[ROWS];
   const int which = threadIdx.x / kLanes, tid = threadIdx.x % kLanes;
   const int row = blockIdx.x * ROWS + which;
   const bool on = row < rows;
   const Part* parts = a.parts + (long long)row * a.segments;
   const int n = on ? a.segments * a.top : 0;
   u64* keys = all_keys[which];
+  if (tid == 0) n_ranked[which] = 0, bound[which] = 0;
   for (int i = tid; i < n; i += kLanes) keys[i] = a.keys[(long long)row * n + i];
   if (on && tid < 64) {
     const long long token = a.token_ids[row];
@@ -348,11 +350,39 @@ __global__ void __launch_bounds__(256) join_kernel(Args a, int rows) {
     }
   }
   __syncthreads();
-  for (int i = tid; i < n; i += kLanes) {
-    const u64 key = keys[i];
+  // Of many keys: the first ones of each segment, `top` in all or a few more, bound the top'th key of the row from below;
+  // what is not below the bound, little more than `top`, is ranked.
+  const bool many = a.segments * a.top > (ROWS == 1 ? 128 : 32);
+  const int leading = (a.top + a.segments - 1) / a.segments, m = on && many ? leading * a.segments : 0;
+  for (int i = tid; i < m; i += kLanes) {
+    const u64 key = keys[i / leading * a.top + i % leading];
+    int ahead = 0;
+#pragma unroll 8
+    for (int j = 0; j < a.segments; ++j)
+      for (int r = 0; r < leading; ++r) ahead += keys[j * a.top + r] > key;
+    if (ahead == a.top - 1 && key) bound[which] = key;
+  }
+  if (many) {
+    __syncthreads();
+    const u64 border = bound[which];
+    for (int i = tid; i < n; i += kLanes) {
+      const u64 key = keys[i];
+      if (key && key >= border) {
+        const int at = atomicAdd(&n_ranked[which], 1);
+        if (at < kRanked) ranked[which][at] = key;
+      }
+    }
+    __syncthreads();
+  }
+  const bool fits = many && n_ranked[which] <= kRanked;
+  const u64* from = fits ? ranked[which] : keys;
+  const int count = fits ? n_ranked[which] : n;
+  for (int i = tid; i < count; i += kLanes) {
+    const u64 key = from[i];
     if (key == 0) continue;  // of a segment with fewer elements than ranks
     int ahead = 0;
-    for (int j = 0; j < n; ++j) ahead += keys[j] > key;
+#pragma unroll 8
+    for (int j = 0; j < count; ++j) ahead += from[j] > key;
     if (ahead < a.top) {
       a.top_ids[(long long)row * a.top + ahead] = index_of(key);
       a.top_logprobs[(long long)row * a.top + ahead] =
