@@ -5,12 +5,14 @@ This is a measurement stand-in for the reference's engine (scheduler, paged atte
 of scope): the non-GEMM pieces are stock PyTorch ops over a contiguous KV cache (RMSNorm, RoPE,
 `scaled_dot_product_attention`, SiLU-and-mul, fp16 lm_head + argmax), weights are synthetic and
 seeded (no checkpoint can be fetched), and one decode step per batch size is captured in a HIP graph
-the way the reference captures its decode batches (vllm/worker/model_runner.py:658-737).
+(`--kv4`: rotation, append and attention are this package's own, over a paged cache that holds keys and values
+in 4 bits; `--logprobs N`: so is the choice of the next token, with its log probability, the entropy and N
+alternatives) the way the reference captures its decode batches (vllm/worker/model_runner.py:658-737).
 Layer order follows vllm/model_executor/models/llama.py:53-80 (MLP), :119-159 (attention), :197-223
 (decoder layer).  tokens/s = batch size / median step time (decode-only variant of
 benchmarks/benchmark_latency.py:59-65).
 
-    python benchmarks/llama_decode.py [--model 7b|70b] [--bs 1,2,4,8,16,32,64] [--layers N]
+    python benchmarks/llama_decode.py [--model 7b|70b] [--bs 1,2,4,8,16,32,64] [--layers N] [--kv4] [--logprobs N]
     torchrun --nproc-per-node 8 benchmarks/llama_decode.py --model 70b      # tensor parallel
     torchrun --nproc-per-node 2 benchmarks/llama_decode.py --backend gloo --same-device --p2p-all-reduce
                                                                             # rehearsal on one GPU
@@ -32,8 +34,9 @@ ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 if ROOT not in sys.path:
     sys.path.insert(0, ROOT)
 
-from vllm_quick_amd._C import ops  # noqa: E402,F401
+from vllm_quick_amd._C import ops  # noqa: E402
 from vllm_quick_amd.layers.activation import gate_up_silu_and_mul  # noqa: E402
+from vllm_quick_amd.layers.kv4_attention import KV4Attention, KV4Metadata, rope_table, slots_of  # noqa: E402
 from vllm_quick_amd.layers.linear import (MergedColumnParallelLinear, QKVParallelLinear,  # noqa: E402
                                           RowParallelLinear, row_parallel_add_)
 from vllm_quick_amd.layers.quantization import AWQConfig  # noqa: E402
@@ -75,9 +78,16 @@ def rope_neox(t, cos2, sin2):
     return torch.addcmul(t * cos2, swapped, sin2)
 
 
+KV4_BLOCK = 16  # tokens of a block of the 4-bit cache
+
+
+def blocks_for(tokens):
+    return -(-tokens // KV4_BLOCK)
+
+
 class DecoderLayer(torch.nn.Module):
 
-    def __init__(self, cfg, method, max_bs, max_len, device):
+    def __init__(self, cfg, method, max_bs, max_len, device, kv4=False):
         super().__init__()
         h, heads, kvh = cfg["hidden"], cfg["heads"], cfg["kv_heads"]
         tp = ps.get_tensor_model_parallel_world_size()
@@ -95,17 +105,24 @@ class DecoderLayer(torch.nn.Module):
         self.fuse_add = True
         self.ln1 = torch.ones(h, dtype=torch.float16, device=device)
         self.ln2 = torch.ones(h, dtype=torch.float16, device=device)
-        self.k_cache = torch.zeros(max_bs, self.n_kv, max_len, self.head_dim, dtype=torch.float16, device=device)
-        self.v_cache = torch.zeros_like(self.k_cache)
+        self.kv4 = KV4Attention(self.n_heads, self.head_dim, self.n_kv) if kv4 else None
+        if kv4:
+            self.kv4_cache = self.kv4.make_cache(max_bs * blocks_for(max_len), KV4_BLOCK, device)
+        else:
+            self.k_cache = torch.zeros(max_bs, self.n_kv, max_len, self.head_dim, dtype=torch.float16, device=device)
+            self.v_cache = torch.zeros_like(self.k_cache)
 
     @staticmethod
     def rms(x, w):
         return rms_norm(x, w)
 
-    def forward(self, x, pos, cos, sin, ctx_len):
+    def forward(self, x, pos, cos, sin, ctx_len, meta=None):
         bs = x.shape[0]
         hdn = self.rms(x, self.ln1)
         qkv, _ = self.qkv_proj(hdn)
+        if self.kv4 is not None:  # (cos: the fp32 table of both)
+            q, k, v = qkv.split([self.n_heads * self.head_dim] + [self.n_kv * self.head_dim] * 2, 1)
+            return self.behind_attention(x, self.kv4(q, k, v, self.kv4_cache, cos, meta))
         nq, nkv, hd = self.n_heads, self.n_kv, self.head_dim
         # rotary embedding on the query and key heads in one pass (they are adjacent in the qkv output)
         qk = rope_neox(qkv[:, :(nq + nkv) * hd].view(bs, nq + nkv, 1, hd), cos, sin)
@@ -115,10 +132,13 @@ class DecoderLayer(torch.nn.Module):
         self.v_cache[:bs, :, pos:pos + 1] = v
         kk, vv = self.k_cache[:bs, :, :ctx_len], self.v_cache[:bs, :, :ctx_len]
         att = F.scaled_dot_product_attention(q, kk, vv, enable_gqa=self.n_kv != self.n_heads)
+        return self.behind_attention(x, att.reshape(bs, -1))
+
+    def behind_attention(self, x, att):
         if self.fuse_add:
-            x = row_parallel_add_(self.o_proj, att.reshape(bs, -1), x)  # x is this step's own buffer
+            x = row_parallel_add_(self.o_proj, att, x)  # x is this step's own buffer
         else:
-            o, _ = self.o_proj(att.reshape(bs, -1))
+            o, _ = self.o_proj(att)
             x = x + o
         hdn = self.rms(x, self.ln2)
         if self.fuse_act:
@@ -147,7 +167,7 @@ class DecoderLayer(torch.nn.Module):
 
 class Model(torch.nn.Module):
 
-    def __init__(self, cfg, n_layers, max_bs, max_len, device, seed=0, keep_stock=True):
+    def __init__(self, cfg, n_layers, max_bs, max_len, device, seed=0, keep_stock=True, kv4=False, logprobs=None):
         super().__init__()
         from vllm_quick_amd.layers.quantization.awq import AWQLinearMethod
         method = AWQLinearMethod(AWQConfig(4, 128, True), keep_stock=keep_stock)
@@ -156,7 +176,7 @@ class Model(torch.nn.Module):
         gen.manual_seed(seed)
         self.layers = torch.nn.ModuleList()
         for _ in range(n_layers):
-            layer = DecoderLayer(cfg, method, max_bs, max_len, device).to(device)
+            layer = DecoderLayer(cfg, method, max_bs, max_len, device, kv4).to(device)
             for lin in (layer.qkv_proj, layer.o_proj, layer.gate_up_proj, layer.down_proj):
                 fill_awq(lin, gen, device)
             self.layers.append(layer)
@@ -169,14 +189,34 @@ class Model(torch.nn.Module):
         t = torch.arange(max_len, device=device).float()
         fr = torch.outer(t, inv)
         self.cos, self.sin = fr.cos().half(), fr.sin().half()
+        self.kv4, self.logprobs = kv4, logprobs
+        if kv4:
+            self.cos_sin = rope_table(max_len, hd, device=device)
+            self.block_tables = torch.arange(max_bs * blocks_for(max_len), dtype=torch.int32, device=device).view(max_bs, -1)
 
-    def step(self, tokens, pos, ctx_len):
+    def kv4_metadata(self, bs, pos, ctx_len):
+        """Every sequence of a batch at position `pos` of its own blocks."""
+        positions = torch.full((bs, ), pos, dtype=torch.int64, device=self.embed.device)
+        tables = self.block_tables[:bs]
+        return KV4Metadata(positions, slots_of(tables, positions, KV4_BLOCK), tables,
+                           torch.full((bs, ), ctx_len, dtype=torch.int32, device=self.embed.device), ctx_len)
+
+    def step(self, tokens, pos, ctx_len, meta=None):
         x = self.embed[tokens]
-        cos, sin = rope_tables(self.cos[pos], self.sin[pos])
-        for layer in self.layers:
-            x = layer(x, pos, cos, sin, ctx_len)
+        if self.kv4:
+            meta = meta or self.kv4_metadata(tokens.shape[0], pos, ctx_len)
+            for layer in self.layers:
+                x = layer(x, pos, self.cos_sin, None, ctx_len, meta)
+        else:
+            cos, sin = rope_tables(self.cos[pos], self.sin[pos])
+            for layer in self.layers:
+                x = layer(x, pos, cos, sin, ctx_len)
         x = DecoderLayer.rms(x, self.norm)
-        return torch.argmax(x @ self.lm_head, -1)
+        if self.logprobs is None:
+            return torch.argmax(x @ self.lm_head, -1)
+        # the likeliest token is the first alternative; its log probability stands with it
+        _, entropy, ids, logprobs = ops.token_logprobs(x @ self.lm_head, tokens, max(1, self.logprobs))
+        return ids[:, 0], logprobs, ids, entropy
 
     def linears_only(self, x):
         for layer in self.layers:
@@ -203,6 +243,7 @@ class Model(torch.nn.Module):
 
 
 def time_graph(fn, stream, reps=20):
+    stream.wait_stream(torch.cuda.current_stream())  # what fn reads was made there
     with torch.cuda.stream(stream):
         for _ in range(2):
             fn()  # warm-up: repacks every layer's weights
@@ -227,7 +268,7 @@ def time_graph(fn, stream, reps=20):
 
 
 def run(model_name="7b", batch_sizes=(1, 2, 4, 8, 16, 32, 64), n_layers=None, ctx_len=128, device=None,
-        fuse_act=True, fuse_add=True, keep_stock=True, rehearse_tp=0):
+        fuse_act=True, fuse_add=True, keep_stock=True, rehearse_tp=0, kv4=False, logprobs=None):
     """`rehearse_tp` = N > 1 on a single process: the step of ONE rank of an N-way tensor-parallel model (layers
     sharded as rank 0's, every all-reduce a device copy of the same size): the compute half of a tensor-parallel
     step, to which a run on N GPUs adds the collectives."""
@@ -236,7 +277,8 @@ def run(model_name="7b", batch_sizes=(1, 2, 4, 8, 16, 32, 64), n_layers=None, ct
     n_layers = n_layers or cfg["layers"]
     rehearsal = ps.rehearse_one_rank(rehearse_tp) if rehearse_tp > 1 else contextlib.nullcontext()
     with torch.inference_mode(), rehearsal:
-        model = Model(cfg, n_layers, max(batch_sizes), ctx_len + 8, device, keep_stock=keep_stock)
+        model = Model(cfg, n_layers, max(batch_sizes), ctx_len + 8, device, keep_stock=keep_stock, kv4=kv4,
+                      logprobs=logprobs)
         for layer in model.layers:
             layer.fuse_act = fuse_act
             layer.fuse_add = fuse_add
@@ -247,7 +289,8 @@ def run(model_name="7b", batch_sizes=(1, 2, 4, 8, 16, 32, 64), n_layers=None, ct
         released = model.drop_stock()
         for bs in batch_sizes:
             tokens = torch.randint(0, cfg["vocab"], (bs, ), device=device)
-            ms = time_graph(lambda: model.step(tokens, ctx_len, ctx_len + 1), stream)
+            meta = model.kv4_metadata(bs, ctx_len, ctx_len + 1) if kv4 else None
+            ms = time_graph(lambda: model.step(tokens, ctx_len, ctx_len + 1, meta), stream)
             xin = (torch.randn(bs, cfg["hidden"], device=device) * 0.25).half()
             ms_lin = time_graph(lambda: model.linears_only(xin), stream)
             scale = cfg["layers"] / n_layers  # extrapolate a reduced-depth run to the full model
@@ -257,7 +300,12 @@ def run(model_name="7b", batch_sizes=(1, 2, 4, 8, 16, 32, 64), n_layers=None, ct
                 "w4a16_gemm_ms": ms_lin * scale,
                 "w4a16_share": ms_lin / ms,
             }
-    return {"model": f"llama-2-{model_name}-awq-shaped (synthetic weights, g128)", "layers_run": n_layers,
+    extra = {}
+    if kv4:
+        extra["kv_cache"] = f"4 bits, blocks of {KV4_BLOCK} tokens"
+    if logprobs is not None:
+        extra["logprobs"] = f"of the chosen token and {max(1, logprobs)} alternative(s)"
+    return {"model": f"llama-2-{model_name}-awq-shaped (synthetic weights, g128)", "layers_run": n_layers, **extra,
             "layers_model": cfg["layers"], "context": ctx_len,
             "tp": rehearse_tp if rehearse_tp > 1 else ps.get_tensor_model_parallel_world_size(),
             "ranks_run": 1 if rehearse_tp > 1 else ps.get_tensor_model_parallel_world_size(),
@@ -280,6 +328,9 @@ def main():
     ap.add_argument("--no-fuse-add", action="store_true", help="add the o_proj / down_proj outputs to the residual "
                     "stream as separate ops")
     ap.add_argument("--drop-stock", action="store_true", help="release the stock AWQ tensors once re-ordered")
+    ap.add_argument("--kv4", action="store_true", help="keys and values in a paged cache of 4 bits, attention over it")
+    ap.add_argument("--logprobs", type=int, default=None, metavar="N",
+                    help="score the chosen token, with N alternatives and the entropy, instead of a bare argmax")
     ap.add_argument("--backend", default="nccl", help="torch.distributed backend: nccl (= RCCL), or gloo for a "
                     "rehearsal (then every all-reduce must take the peer-to-peer path)")
     ap.add_argument("--same-device", action="store_true", help="rehearsal: every rank uses GPU 0")
@@ -316,7 +367,8 @@ def main():
     from vllm_quick_amd.parallel_utils import rccl_utils as direct
     with (ps.with_rccl_for_all_reduce() if direct.is_initialized() else contextlib.nullcontext()):
         out = run(a.model, tuple(int(v) for v in a.bs.split(",")), a.layers or None, a.ctx,
-                  fuse_act=not a.no_fuse_act, fuse_add=not a.no_fuse_add, keep_stock=not a.drop_stock)
+                  fuse_act=not a.no_fuse_act, fuse_add=not a.no_fuse_add, keep_stock=not a.drop_stock, kv4=a.kv4,
+                  logprobs=a.logprobs)
     out["wall_s"] = time.time() - t0
     out["all_reduce"] = "peer-to-peer kernel" if world > 1 and a.p2p_all_reduce else ("rccl" if world > 1 else None)
     if world > 1 and a.p2p_all_reduce:

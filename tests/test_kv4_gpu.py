@@ -448,6 +448,7 @@ def test_captured_steps_replay(ops, cuda):
     side = torch.cuda.Stream()
     for _ in range(2):
         st = make()
+        side.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(side):
             step(st)
             side.synchronize()
