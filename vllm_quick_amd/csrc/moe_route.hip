@@ -78,7 +78,11 @@ __global__ void __launch_bounds__(256) moe_combine_kernel(const f16* __restrict_
     if (w == 0.f) continue;
     const f16x8 v = *reinterpret_cast<const f16x8*>(y + ((size_t)e * tokens + t) * hidden + (size_t)c * 8);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) acc[i] += (float)(f16)((float)v[i] * w);
+    for (int i = 0; i < 8; ++i) {
+      float product = (float)v[i] * w;
+      asm("" : "+v"(product));  // (rounded to fp32, then to fp16: one instruction would do both at once)
+      acc[i] += (float)(f16)product;
+    }
   }
   f16x8 r;
 #pragma unroll
