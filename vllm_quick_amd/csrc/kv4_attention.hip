@@ -95,7 +95,7 @@ __device__ __forceinline__ Sequence sequence(const AttendArgs& a, int b) {
   return s;
 }
 
-template <typename T, int D, int NC>
+template <typename T, int D, int NC, bool ONCE>
 struct Wave {
   static constexpr int kSteps = D / 32;  // matrix instructions of 16 keys against 16 columns
   static constexpr int kRows = D / 16;   // tiles of 16 elements of the result
@@ -217,16 +217,23 @@ struct Wave {
     }
   }
 
+  // Where each key is read once (ONCE: one column tile) the codes pass the caches by: 8 x 65536 keys 82 us against 91.
+  // (The parameters of several tiles share a line.)
+  template <typename V>
+  static __device__ __forceinline__ V get(const uint8_t* at) {
+    return ONCE ? __builtin_nontemporal_load(reinterpret_cast<const V*>(at)) : *reinterpret_cast<const V*>(at);
+  }
+
   __device__ __forceinline__ void load_keys() {
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       const uint8_t* at = base[s] + (uint32_t)(place[s] * Kv4<D>::kTokenBytes) + (uint32_t)(c * Kv4<D>::kTokenBytes + g * (D / 8));
       if (D == 128) {
-        const u32x4 w = *reinterpret_cast<const u32x4*>(at);
+        const u32x4 w = get<u32x4>(at);
 #pragma unroll
         for (int j = 0; j < kSteps; ++j) k[s][j] = w[j];
       } else {
-        const u32x2 w = *reinterpret_cast<const u32x2*>(at);
+        const u32x2 w = get<u32x2>(at);
 #pragma unroll
         for (int j = 0; j < kSteps; ++j) k[s][j] = w[j];
       }
@@ -246,8 +253,8 @@ struct Wave {
     const int piece = D == 128 ? c : c >> 1;
 #pragma unroll
     for (int s = 0; s < 2; ++s)
-      v[s] = *reinterpret_cast<const u32x4*>(base[s] + (uint32_t)(Kv4<D>::values(a.block_size) + (place[s] / 16) * Kv4<D>::kGroupBytes) +
-                                             (uint32_t)(piece * Kv4<D>::kPieceBytes + 16 * g));
+      v[s] = get<u32x4>(base[s] + (uint32_t)(Kv4<D>::values(a.block_size) + (place[s] / 16) * Kv4<D>::kGroupBytes) +
+                        (uint32_t)(piece * Kv4<D>::kPieceBytes + 16 * g));
   }
 
   __device__ __forceinline__ bool sees(int n, int from, int i) const {
@@ -487,7 +494,7 @@ __global__ void __launch_bounds__(64 * WAVES, NC == 1 ? 3 : 2) attend_split_kern
   const int pair = blockIdx.x, b = pair / a.kv_heads, kv = pair - b * a.kv_heads;
   const int split = blockIdx.y, tile = blockIdx.z;
   const int per_piece = a.chunk / kTile;
-  Wave<T, D, NC> w(a);
+  Wave<T, D, NC, NC == 1> w(a);  // (16 columns are all there are)
   // Without a window a piece begins where it does whatever the length, which is under way meanwhile: one round trip to
   // memory less before the first keys.
   if (a.window == 0) w.first_loads(b, kv, split * per_piece + wave, &part[wave][0][0]);
@@ -637,7 +644,7 @@ __global__ void __launch_bounds__(256, 2) attend_prompt_kernel(AttendArgs a) {
   const int col0 = (groups - 1 - (int)blockIdx.y) * group_cols + wave * kCols;
   if (col0 >= cols) return;
   const Range r = range(a, s, col0, min(cols - 1, col0 + kCols - 1));
-  Wave<T, D, NC> w(a);
+  Wave<T, D, NC, false> w(a);
   w.first_loads(b, kv, r.first_tile, &part[wave][0][0]);
   w.begin(s, kv, col0, cols);
   w.run(r.first_tile, r.last_tile, 1, s.length, r.whole_from, r.whole_to);
