@@ -66,7 +66,9 @@ def check_append(ops, cuda, case, interleaved, d):
     (65, 3, 3, 64, 4096, 48, False),
     (19, 5, 5, 128, 16, 0, False),
     (511, 4, 2, 128, 16, 128, False),
-    (512, 4, 2, 128, 16, 128, True),  # sixteen tokens a workgroup from here
+    (512, 4, 2, 128, 16, 128, True),
+    (77, 1, 1, 64, 16, 64, False),  # sixteen tokens a workgroup
+    (13, 70, 7, 64, 16, 64, True),  # several passes over a token's heads
     (1000, 6, 3, 64, 32, 64, False),
 ])
 def test_append(ops, cuda, t, heads, kv, d, p, rotary, interleaved, dtype):
