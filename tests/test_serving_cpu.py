@@ -257,3 +257,27 @@ def test_oracle_attention_is_torchs():
     want = torch.nn.functional.scaled_dot_product_attention(q.double().transpose(0, 1), k.transpose(0, 1).expand(2, n, d),
                                                             v.transpose(0, 1).expand(2, n, d), is_causal=True, scale=0.1)
     assert torch.allclose(got, want.transpose(0, 1), rtol=1e-12, atol=1e-12)
+
+
+def test_more_than_a_grid_holds_is_refused(lib):
+    assert append(lib, tokens=1 << 26) == -8
+
+
+@pytest.mark.parametrize("change,text", [
+    (dict(query=torch.zeros(3, 0, 128, dtype=torch.float16)), "0 heads"),  # (its keys would not be stored)
+    (dict(cos_sin=torch.zeros(0, 128)), "no positions"),
+])
+def test_append_operator_refuses_nothing_to_rotate_by(ops, change, text):
+    with pytest.raises(ValueError, match=text):
+        ops.rope_append_kv4(**append_args(**change))
+
+
+def test_slots_of_positions():
+    """Rows of a padded batch (position -1), positions past the table and pages without a block have no slot."""
+    from vllm_quick_amd.layers.kv4_attention import slots_of
+    tables = torch.tensor([[5, 2], [7, -1], [0, 0]], dtype=torch.int32)
+    got = slots_of(tables, torch.tensor([17, 3, -1]), 16)
+    assert got.tolist() == [2 * 16 + 1, 7 * 16 + 3, -1]
+    got = slots_of(tables, torch.tensor([0, 31, 32, 15, 16, 10**9]), 16, torch.tensor([0, 0, 0, 1, 1, 2]))
+    assert got.tolist() == [80, 47, -1, 127, -1, -1]
+    assert slots_of(tables[:, :0], torch.tensor([0, 1, -1]), 16).tolist() == [-1, -1, -1]

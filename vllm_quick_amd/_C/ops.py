@@ -743,7 +743,7 @@ def paged_attention_kv4(query: torch.Tensor, cache: torch.Tensor, block_tables: 
     query_start (int32 [sequences + 1]) rows query_start[b] .. query_start[b + 1] - 1 are the last tokens of sequence b
     and each sees what stands up to itself; window > 0: the last `window` of that.  max_seq_len and max_query_len size
     the launch; rows past max_query_len of a sequence come back NaN.  A row that sees nothing is zero; rows of no
-    sequence are left as `out` holds them."""
+    sequence are left as `out` holds them.  `out` may be the query itself."""
     return _native.paged_attention_kv4(query, cache, block_tables, seq_lens, scale, max_seq_len, query_start, max_query_len,
                                        window, out)
 

@@ -277,6 +277,7 @@ extern "C" int serving_rope_append_kv4(const void* query, long long q_token, lon
   int per_pass = kThreads / (head_size / 16);  // heads of a token that a workgroup takes at once
   while (per_pass >= 2 * all) per_pass /= 2, ++a.token_shift;
   const int x = (tokens + (1 << a.token_shift) - 1) >> a.token_shift;
+  if (x > 0xffffff) return SERVING_E_TOO_LARGE;  // (a grid has less than 2^32 threads in a direction)
   const int passes = (all + per_pass - 1) / per_pass;
   // as many workgroups as fill the chip a few times over, and no more: each reads its token's angles once
   int y = (2048 + x - 1) / x;
@@ -309,7 +310,7 @@ extern "C" int serving_read_kv4(const void* cache, const int64_t* slots, void* k
   if (rows > (1LL << 40)) return SERVING_E_TOO_LARGE;
   const long long pieces = rows * kv_heads * (head_size / 8);
   const long long groups = (pieces + kThreads - 1) / kThreads;
-  if (groups > 0x7fffffffLL) return SERVING_E_TOO_LARGE;
+  if (groups > 0xffffff) return SERVING_E_TOO_LARGE;
   const dim3 grid((unsigned)groups);
   hipStream_t s = static_cast<hipStream_t>(stream);
   const uint8_t* c = static_cast<const uint8_t*>(cache);

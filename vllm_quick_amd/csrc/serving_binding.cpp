@@ -2,6 +2,7 @@
 // allocator, torch's current stream, a device guard.  No kernel here, nothing is kept between calls, nothing is
 // synchronised: every call may be captured in a graph.  ValueError for shapes, RuntimeError for types and devices, as
 // the AWQ operators have it.
+#include <ATen/MemoryOverlap.h>
 #include <ATen/core/grad_mode.h>
 #include <ATen/hip/HIPContext.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
@@ -112,7 +113,8 @@ Tensor rope_append_kv4(const Tensor& positions, const Tensor& query, const Tenso
   NEED(cos_sin.dim() == 2, "cos_sin must be [positions, rotary], got ", shape_of(cos_sin));
   const int64_t rotary = cos_sin.size(1);
   NEED(rotary % 16 == 0 && rotary <= d, "the rotated part of a head must be a multiple of 16 elements and no larger than a head, got ", rotary);
-  NEED(tokens <= (1 << 30) && heads <= 65535, "too many tokens or heads");
+  NEED(rotary == 0 || cos_sin.size(0) > 0, "cos_sin has no positions");
+  NEED(tokens <= (1 << 30) && heads > 0 && heads <= 65535, "query has too many tokens, or ", heads, " heads");
   for (const auto& [t, name] : {std::pair<const Tensor&, const char*>(query, "query"), {key, "key"}, {value, "value"},
                                 {cos_sin, "cos_sin"}, {cache, "cache"}, {positions, "positions"}, {slots, "slots"}}) {
     on_gpu(t, query, what, name);
@@ -120,7 +122,7 @@ Tensor rope_append_kv4(const Tensor& positions, const Tensor& query, const Tenso
   }
   const OptionalHIPGuardMasqueradingAsCUDA guard(query.device());
   Tensor out = torch::empty({tokens, heads, d}, query.options());
-  if (tokens == 0 || heads == 0) return out;
+  if (tokens == 0) return out;
   const Tensor q = heads_of(query), k = heads_of(key), v = heads_of(value), at = ints(positions), to = ints(slots);
   const bool table_fits = rotary == 0 || (cos_sin.stride(1) == 1 && cos_sin.stride(0) % 4 == 0 &&
                                           reinterpret_cast<uintptr_t>(cos_sin.data_ptr()) % 16 == 0);
@@ -192,6 +194,8 @@ Tensor paged_attention_kv4(const Tensor& query, const Tensor& cache, const Tenso
     no_gradient(*out_, what, "out");
     NEED(out_->sizes() == query.sizes() && out_->is_contiguous(), "out must be a contiguous ", shape_of(query), ", got ", shape_of(*out_));
     TORCH_CHECK(reinterpret_cast<uintptr_t>(out_->data_ptr()) % 16 == 0, what, ": out is not 16-byte aligned");
+    at::assert_no_partial_overlap(*out_, query);
+    at::assert_no_overlap(*out_, cache);
   }
   const OptionalHIPGuardMasqueradingAsCUDA guard(query.device());
   Tensor out = out_ ? *out_ : torch::empty({tokens, heads, d}, query.options());

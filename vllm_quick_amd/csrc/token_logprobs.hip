@@ -453,7 +453,7 @@ extern "C" int serving_token_logprobs(const void* logits, long long row_stride, 
   const int bytes = type == 2 ? 4 : 2;
   if (reinterpret_cast<uintptr_t>(logits) % bytes) return SERVING_E_ALIGN;
   const Plan p = plan(rows, vocab, type);
-  if ((long long)rows * p.segments > 0x7fffffffLL) return SERVING_E_TOO_LARGE;
+  if ((long long)rows * p.segments * p.threads > 0xffffffffLL) return SERVING_E_TOO_LARGE;
   const size_t need = serving_token_logprobs_workspace_bytes(rows, vocab, top, type);
   if (need && (!workspace || workspace_bytes < need)) return SERVING_E_WORKSPACE;
   if (need && !aligned16(workspace)) return SERVING_E_ALIGN;

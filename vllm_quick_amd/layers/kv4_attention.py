@@ -30,10 +30,15 @@ class KV4Metadata:
 def slots_of(block_tables: torch.Tensor, positions: torch.Tensor, block_size: int,
              sequences: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Slots of tokens at `positions` of their sequences (row of block_tables for each token; None: token i is of sequence
-    i): block * block_size + place in the block."""
+    i): block * block_size + place in the block; -1, which stores nothing, for a position that the row has no block for
+    (a padded token's -1)."""
     rows = block_tables if sequences is None else block_tables[sequences]
-    block = rows.long().gather(1, (positions // block_size)[:, None])[:, 0]
-    return block * block_size + positions % block_size
+    if rows.shape[1] == 0:
+        return torch.full_like(positions, -1)
+    page = torch.div(positions, block_size, rounding_mode="floor")
+    block = rows.long().gather(1, page.clamp(0, rows.shape[1] - 1)[:, None])[:, 0]
+    held = (page >= 0) & (page < rows.shape[1]) & (block >= 0)
+    return torch.where(held, block * block_size + positions % block_size, -1)
 
 
 def rope_table(positions: int, rotary: int, base: float = 10000.0, device: Optional[torch.device] = None) -> torch.Tensor:
