@@ -1,0 +1,177 @@
+"""Attention over the 4-bit cache where a sequence has many columns (queries x heads of a kv head): batches large enough
+that each wave takes columns of its own, and those of few or uneven rows, where waves share the keys."""
+import pytest
+import torch
+
+from oracle import serving_oracle as orc
+from test_kv4_gpu import TYPES, attend_case, check_attend
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from vllm_quick_amd import ops
+    return ops
+
+
+def in_a_large_batch(case, tiles):
+    """The case with rows of no sequence behind it, so many that the batch counts as one that fills the chip."""
+    query, *rest = case
+    rows = max(0, -(-tiles * 32 // query.shape[1]) - query.shape[0])
+    return torch.cat([query, torch.ones(rows, *query.shape[1:], dtype=query.dtype)]), *rest
+
+
+def check_in_a_large_batch(ops, cuda, case, tiles=2048, **kw):
+    case = in_a_large_batch(case, tiles)
+    out = torch.full(case[0].shape, 7.0, dtype=case[0].dtype, device=cuda)
+    got = check_attend(ops, cuda, case, out=out, **kw)
+    assert (got[int(case[4][-1]):] == 7.0).all()
+    return got
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("lens,counts,heads,kv,d,p", [
+    ([65], [65], 3, 3, 64, 16),
+    ([100, 37], [100, 37], 2, 2, 128, 16),
+    ([333], [129], 6, 2, 64, 48),                       # 387 columns: a workgroup's last wave has a few
+    ([400, 1, 257], [130, 1, 257], 8, 1, 128, 32),
+    ([3, 90], [40, 9], 8, 4, 128, 16),                  # more queries than tokens: rows that see nothing
+    ([0, 200, 50], [33, 40, 0], 4, 2, 64, 16),
+    ([90, 17], [1, 1], 130, 2, 128, 16),                # single tokens of many heads
+    ([1500], [70], 2, 2, 64, 16),                       # set aside in between
+])
+@pytest.mark.parametrize("window", [0, 1, 40])
+def test_columns_of_their_own(ops, cuda, lens, counts, heads, kv, d, p, dtype, window):
+    check_in_a_large_batch(ops, cuda, attend_case(lens, counts, heads, kv, d, p, TYPES[dtype], seed=sum(lens)), window=window)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("window", [0, 1300])
+def test_columns_of_their_own_over_long_sequences(ops, cuda, dtype, window):
+    check_in_a_large_batch(ops, cuda, attend_case([2500, 2200], [40, 33], 4, 2, 128, 64, TYPES[dtype], 61), 4096, window=window)
+
+
+def test_columns_of_their_own_of_many_sequences(ops, cuda):
+    """More sequences than are ordered by their length, and as many as are."""
+    g = torch.Generator().manual_seed(5)
+    for seqs in (64, 70):
+        counts = torch.randint(0, 34, (seqs, ), generator=g).tolist()
+        lens = [c + int(x) for c, x in zip(counts, torch.randint(0, 50, (seqs, ), generator=g))]
+        counts[3] = 33
+        check_in_a_large_batch(ops, cuda, attend_case(lens, counts, 2, 1, 64, 16, torch.float16, seqs))
+
+
+def test_columns_of_their_own_do_not_see_what_stands_behind(ops, cuda):
+    d, p = 128, 16
+    query, cache, tables, lens, start = in_a_large_batch(attend_case([100, 90], [40, 70], 4, 2, d, p, torch.float16, 31), 2048)
+    run = lambda c, t: ops.paged_attention_kv4(query.to(cuda), c.to(cuda), t.to(cuda), lens.to(cuda), 0.1, 128,  # noqa: E731
+                                               query_start=start.to(cuda), max_query_len=70).cpu()[:110]
+    base = run(cache, tables)
+    slot = (tables[1].long()[89 // p] * p + 89 % p).view(1)
+    for x in (float("nan"), 60000.0):
+        other = cache.clone()
+        orc.store(other, d, slot, torch.full((1, 2, d), x), torch.full((1, 2, d), x))
+        got = run(other, tables)
+        assert torch.equal(got[:109], base[:109]) and not torch.isnan(base[:109]).any()
+        assert torch.isnan(got[109]).all() or x == x
+    for bad in (-1, cache.shape[0], 2**31 - 1):  # a block of its last 26 tokens that does not exist
+        wrong = tables.clone()
+        wrong[1, 4] = bad
+        got = run(cache, wrong)
+        seen = 40 + 70 - 26
+        assert torch.equal(got[:seen], base[:seen]) and torch.isnan(got[seen:]).all()
+
+
+@pytest.mark.parametrize("large", [False, True])
+def test_rows_past_the_promise_among_many(ops, cuda, large):
+    case = attend_case([300, 90], [43, 20], 4, 1, 64, 16, torch.bfloat16, 41)
+    query, cache, tables, lens, start = in_a_large_batch(case, 2048) if large else case
+    out = torch.full(query.shape, 7.0, dtype=query.dtype, device=cuda)
+    ops.paged_attention_kv4(query.to(cuda), cache.to(cuda), tables.to(cuda), lens.to(cuda), 0.125, 300,
+                            query_start=start.to(cuda), max_query_len=30, out=out)
+    want, tol = orc.attend(query, cache, tables, lens, start, 0.125, 0, False)
+    got = out.cpu().double()
+    kept = list(range(30)) + list(range(43, 63))
+    assert ((got - want).abs() <= tol)[kept].all() and torch.isnan(got[30:43]).all() and (got[63:] == 7.0).all()
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("lens,counts,heads,kv,d,p,window", [
+    ([5000], [1], 128, 1, 128, 64, 0),                  # one token of many heads, in pieces
+    ([3000, 700], [50, 40], 4, 2, 64, 16, 0),           # rows of a prompt, in pieces
+    ([3000, 700], [50, 40], 4, 2, 64, 16, 900),
+    ([600, 900, 33, 0, 700], [200, 1, 1, 0, 1], 8, 2, 128, 32, 0),  # one prompt with single tokens
+    ([600, 900, 33, 0, 700], [200, 1, 1, 0, 1], 8, 2, 128, 32, 100),
+    ([1, 50, 2], [1, 50, 1], 66, 33, 64, 16, 0),
+])
+def test_few_rows_share_the_keys(ops, cuda, lens, counts, heads, kv, d, p, window, dtype):
+    check_attend(ops, cuda, attend_case(lens, counts, heads, kv, d, p, TYPES[dtype], seed=sum(lens)), window=window)
+
+
+def test_both_ways_agree(ops, cuda):
+    """The same rows alone and in a large batch: within what either may be off."""
+    case = attend_case([700, 300], [90, 80], 4, 2, 128, 16, torch.bfloat16, 71)
+    alone = check_attend(ops, cuda, case)
+    among = check_in_a_large_batch(ops, cuda, case)[:170]
+    _, tol = orc.attend(*case, 128**-0.5, 0, False)
+    assert ((alone.cpu().double() - among.cpu().double()).abs() <= 2 * tol).all()
+
+
+def test_out_may_be_the_query(ops, cuda):
+    for lens, counts, tiles in (([300, 40], [1, 1], 0), ([5000], [1], 0), ([300], [90], 0), ([300], [90], 2048)):
+        query, cache, tables, lens_, start = in_a_large_batch(attend_case(lens, counts, 4, 2, 64, 16, torch.float16, 73), tiles)
+        q, args = query.to(cuda), [x.to(cuda) for x in (cache, tables, lens_)]
+        kw = dict(query_start=start.to(cuda), max_query_len=max(counts))
+        rows = int(start[-1])
+        want = ops.paged_attention_kv4(q, *args, 0.1, max(lens), **kw)[:rows]
+        assert ops.paged_attention_kv4(q, *args, 0.1, max(lens), out=q, **kw).data_ptr() == q.data_ptr()
+        assert torch.equal(q[:rows], want) and torch.equal(q[rows:].cpu(), query[rows:])
+    both = torch.zeros(3, 4, 64, dtype=torch.float16, device=cuda)
+    with pytest.raises(RuntimeError, match="single memory location"):
+        ops.paged_attention_kv4(both[:2], *args[:1], torch.zeros(2, 1, dtype=torch.int32, device=cuda),
+                                torch.ones(2, dtype=torch.int32, device=cuda), 0.1, 1, out=both[1:])
+
+
+def test_outs_that_are_refused(ops, cuda):
+    query, cache, tables, lens, start = [x.to(cuda) for x in attend_case([30, 4], [1, 1], 4, 2, 64, 16, torch.float16, 79)]
+    args = (query, cache, tables, lens, 0.1, 30)
+    for out, error, text in ((query[:1].clone(), ValueError, "out must be"), (query.float(), RuntimeError, "out"),
+                             (torch.empty(2, 64, 4, dtype=query.dtype, device=cuda).transpose(1, 2), ValueError, "contiguous"),
+                             (torch.empty(513, dtype=query.dtype, device=cuda)[1:].view(2, 4, 64), RuntimeError, "aligned"),
+                             (query.cpu(), RuntimeError, "GPU tensor")):
+        with pytest.raises(error, match=text):
+            ops.paged_attention_kv4(*args, out=out)
+
+
+def test_gradients_are_refused(ops, cuda):
+    query, cache, tables, lens, start = [x.to(cuda) for x in attend_case([30, 4], [1, 1], 4, 2, 64, 16, torch.float16, 83)]
+    slots = torch.zeros(2, dtype=torch.int64, device=cuda)
+    slots[1] = 40
+    kv = torch.zeros(2, 2, 64, dtype=torch.float16, device=cuda)
+    cs = torch.zeros(1, 64, device=cuda)
+    calls = [lambda q: ops.paged_attention_kv4(q, cache, tables, lens, 0.1, 30),
+             lambda q: ops.rope_append_kv4(slots, q, kv, kv, cs, cache, slots),
+             lambda q: ops.token_logprobs(q.view(2, -1), slots, 1)]
+    for call in calls:
+        leaf = query.clone().requires_grad_()
+        with pytest.raises(RuntimeError, match="requires a gradient"):
+            call(leaf)
+        with torch.no_grad():
+            call(leaf)
+
+
+def test_tables_without_a_block(ops, cuda):
+    """No sequence has a block: every row of single tokens sees nothing; of other batches nobody knows where rows are."""
+    query, cache, tables, lens, start = [x.to(cuda) for x in attend_case([30, 4], [1, 1], 4, 2, 64, 16, torch.float16, 89)]
+    assert (ops.paged_attention_kv4(query, cache, tables[:, :0], lens, 0.1, 30) == 0).all()
+    with pytest.raises(ValueError, match="no columns"):
+        ops.paged_attention_kv4(query, cache, tables[:, :0], lens, 0.1, 30, query_start=start)
+
+
+def test_one_cache_serves_both_types(ops, cuda):
+    """What an fp16 caller appended a bf16 caller attends to, to the same values."""
+    query, cache, tables, lens, start = attend_case([200, 70], [1, 1], 4, 2, 128, 16, torch.bfloat16, 97)
+    small = torch.round(query.float() * 8) / 8  # (of few enough digits for either type)
+    for dtype in TYPES.values():
+        check_attend(ops, cuda, (small.to(dtype), cache, tables, lens, start), ragged=False)

@@ -492,12 +492,15 @@ __global__ void __launch_bounds__(64 * WAVES, NC == 1 ? 3 : 2) attend_split_kern
   __shared__ float maxima[WAVES][kCols], sums[WAVES][kCols];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int pair = blockIdx.x, b = pair / a.kv_heads, kv = pair - b * a.kv_heads;
-  const int split = blockIdx.y, tile = blockIdx.z;
+  const int split = blockIdx.y;
+  const int tile = gridDim.z - 1 - blockIdx.z;  // (those that see most come first)
   const int per_piece = a.chunk / kTile;
   Wave<T, D, NC, NC == 1> w(a);  // (16 columns are all there are)
   // Without a window a piece begins where it does whatever the length, which is under way meanwhile: one round trip to
   // memory less before the first keys.
-  if (a.window == 0) w.first_loads(b, kv, split * per_piece + wave, &part[wave][0][0]);
+  // (Where most workgroups may find no queries to work on they ask first.)
+  const bool ahead = a.window == 0 && gridDim.z <= 2;
+  if (ahead) w.first_loads(b, kv, split * per_piece + wave, &part[wave][0][0]);
   const Sequence s = sequence(a, b);
   const int queries = min(s.queries, a.max_query_len), cols = queries * a.group;
   if (tile == 0 && split == 0 && queries < s.queries) refuse_rows<T, D>(a, s, kv);
@@ -508,7 +511,7 @@ __global__ void __launch_bounds__(64 * WAVES, NC == 1 ? 3 : 2) attend_split_kern
   if (split >= pieces) return;
   const int t0 = r.first_tile + split * per_piece + wave;
   const int t1 = split == pieces - 1 ? r.last_tile : r.first_tile + (split + 1) * per_piece;
-  if (a.window > 0) w.first_loads(b, kv, t0, &part[wave][0][0]);
+  if (!ahead) w.first_loads(b, kv, t0, &part[wave][0][0]);
   w.begin(s, kv, col0, cols);
   w.run(t0, t1, WAVES, s.length, r.whole_from, r.whole_to);
 
@@ -676,17 +679,27 @@ struct Plan {
   bool prompt;
   int nc, tiles, waves, splits, chunk;
 };
-Plan plan(int seqs, int heads, int kv_heads, int max_query_len, int max_seq_len, int window) {
-  const long long cols = (long long)max_query_len * (heads / kv_heads);
+Plan plan(int tokens, int seqs, int heads, int kv_heads, int max_query_len, int max_seq_len, int window) {
+  const long long group = heads / kv_heads, cols = max_query_len * group;
   Plan p;
-  p.prompt = cols > 64;
   p.nc = cols > 16 ? 2 : 1;
   p.tiles = (int)((cols + 16 * p.nc - 1) / (16 * p.nc));
   p.waves = 4;
   p.splits = 1;
   p.chunk = 1 << 27;
+  // Column tiles that hold queries: of all rows together (a batch may mix one prompt with many single tokens), a tile a
+  // sequence more where they do not fill their last.
+  const long long full = (tokens * group + 16 * p.nc - 1) / (16 * p.nc);
+  const long long most_tiles = (long long)seqs * p.tiles, tiles = full + seqs < most_tiles ? full + seqs : most_tiles;
+  // A wave for each column tile where these alone fill the chip, two waves a SIMD, and the rows are spread about evenly:
+  // 2 x 8 kv heads x 1024 queries of 8 heads take 70 us so and 98 with waves that share the keys, 64 x 8 x 32 queries of
+  // 4 heads over 1024 keys 60 and 71.  Below that some SIMDs idle while others have all the keys to run over: one
+  // sequence's 512 queries of 8 x 4 heads over 8192 keys 268 and 102, one query of 128 heads over 65536 keys 2070 and 29;
+  // 2048 queries beside 63 single ones, each over 4096 keys, 995 and 705.  Long sequences want a second such round
+  // (2048 queries of 8 x 4 heads over 65536 keys, one round: 2970 and 2710; twice 2048 over 8192, two: 633 and 630).
+  p.prompt = cols > 64 && full * kv_heads >= (max_seq_len > 2048 ? 4096 : 2048) && 2 * full >= most_tiles;
   if (p.prompt) return p;
-  const long long groups = (long long)seqs * kv_heads * p.tiles;
+  const long long groups = tiles * kv_heads;
   long long keys = max_seq_len;
   if (window > 0 && (long long)window + max_query_len < keys) keys = window + max_query_len;
   // Where a workgroup a CU is all there is, eight waves share up to 2048 keys and no second kernel runs: 16 x 4 kv heads
@@ -695,7 +708,7 @@ Plan plan(int seqs, int heads, int kv_heads, int max_query_len, int max_seq_len,
   // (the last round of workgroups leaves most CUs idle), 115 in 48.
   if (groups * ((keys + 2047) / 2048) <= 256) p.waves = 8;
   const long long least = p.waves == 8 ? 2048 : 512, most = (keys + least - 1) / least;
-  long long splits = (p.waves == 8 ? 256 : 768) / groups;
+  long long splits = (p.waves == 8 ? 256 : p.nc == 2 ? 512 : 768) / groups;
   splits = splits < most ? splits : most;
   splits = splits < 1 ? 1 : splits > 64 ? 64 : splits;
   if (splits == 1) return p;
@@ -744,7 +757,7 @@ bool sizes_ok(int tokens, int seqs, int heads, int kv_heads, int max_query_len, 
 extern "C" size_t serving_attend_kv4_workspace_bytes(int tokens, int seqs, int heads, int kv_heads, int head_size,
                                                      int max_query_len, int max_seq_len, int window) {
   if (!sizes_ok(tokens, seqs, heads, kv_heads, max_query_len, max_seq_len, window) || !head_size_ok(head_size)) return 0;
-  const Plan p = plan(seqs, heads, kv_heads, max_query_len, max_seq_len, window);
+  const Plan p = plan(tokens, seqs, heads, kv_heads, max_query_len, max_seq_len, window);
   return p.splits == 1 ? 0 : (size_t)tokens * heads * p.splits * (head_size + 2) * sizeof(float);
 }
 
@@ -763,12 +776,13 @@ extern "C" int serving_attend_kv4(const void* query, long long q_token, long lon
     return SERVING_E_SHAPE;
   if ((long long)table_width * block_size > (1LL << 27)) return SERVING_E_TOO_LARGE;
   if (!aligned16(query) || !aligned16(cache) || !aligned16(out) || q_token % 8 || q_head % 8) return SERVING_E_ALIGN;
-  const Plan p = plan(seqs, heads, kv_heads, max_query_len, max_seq_len, window);
+  const Plan p = plan(tokens, seqs, heads, kv_heads, max_query_len, max_seq_len, window);
+  if ((long long)seqs * kv_heads > 0x7fffffLL || (p.prompt && seqs > 65535) || p.tiles > (p.prompt ? 4 : 1) * 65535LL ||
+      (long long)tokens * heads > (p.splits > 1 ? 0x3ffffffLL : 0x7fffffffLL))
+    return SERVING_E_TOO_LARGE;
   const size_t need = serving_attend_kv4_workspace_bytes(tokens, seqs, heads, kv_heads, head_size, max_query_len, max_seq_len, window);
   if (need && (!workspace || workspace_bytes < need)) return SERVING_E_WORKSPACE;
   if (need && !aligned16(workspace)) return SERVING_E_ALIGN;
-  if ((long long)seqs * kv_heads > 0x7fffffLL || (p.prompt && seqs > 65535) || p.tiles > 4 * 65535LL || (long long)tokens * heads > 0x7fffffffLL)
-    return SERVING_E_TOO_LARGE;
   const int sixteens = block_size / 16;
   AttendArgs a{query, q_token, q_head, static_cast<const uint8_t*>(cache), tables, table_stride, seq_lens, query_start, out,
                static_cast<float*>(workspace), nullptr, table_width, tokens, seqs, heads, kv_heads, heads / kv_heads,
