@@ -175,3 +175,46 @@ def test_one_cache_serves_both_types(ops, cuda):
     small = torch.round(query.float() * 8) / 8  # (of few enough digits for either type)
     for dtype in TYPES.values():
         check_attend(ops, cuda, (small.to(dtype), cache, tables, lens, start), ragged=False)
+
+
+@pytest.mark.parametrize("seqs,kv,longest,window", [
+    (200, 1, 3000, 0), (200, 1, 3000, 700),  # more sequences than lanes
+    (70, 4, 700, 0), (64, 4, 5000, 0), (130, 1, 2500, 0),
+    (300, 4, 900, 0),                        # too many to be cut
+])
+def test_one_long_sequence_among_short_ones(ops, cuda, seqs, kv, longest, window):
+    """It comes in pieces wherever it stands, the others in one, those without a token in none that count."""
+    for at in (0, seqs // 2, seqs - 1):
+        lens = [(7 * i) % 40 for i in range(seqs)]
+        lens[at] = longest
+        case = attend_case(lens, [1] * seqs, 2 * kv, kv, 64, 16, torch.float16, seqs + at)
+        check_attend(ops, cuda, case, window=window, ragged=False)
+
+
+def test_a_prompt_among_tokens_in_pieces(ops, cuda):
+    lens, counts = [40] * 36, [1] * 36
+    lens[5], counts[5], lens[20], counts[20], counts[30] = 3000, 90, 1300, 3, 0
+    for window in (0, 1000):
+        check_attend(ops, cuda, attend_case(lens, counts, 16, 8, 64, 16, torch.bfloat16, 101), window=window)
+
+
+def test_a_captured_step_of_sequences_that_grow(ops, cuda):
+    """Captured for the longest sequence there may be: each replay cuts what it finds into pieces anew."""
+    case = attend_case([6000, 1, 300, 40], [1] * 4, 8, 2, 128, 16, torch.float16, 103)
+    query, cache, tables, _, start = [x.to(cuda) for x in case]
+    lens = torch.ones(4, dtype=torch.int32, device=cuda)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        ops.paged_attention_kv4(query, cache, tables, lens, 0.1, 6000)
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = ops.paged_attention_kv4(query, cache, tables, lens, 0.1, 6000)
+    for now in ([1, 1, 1, 1], [6000, 1, 300, 40], [900, 0, 5, 40], [4097, 1, 299, 0]):
+        lens.copy_(torch.tensor(now, dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        want, tol = orc.attend(case[0], case[1], case[2], torch.tensor(now), case[4], 0.1, 0, True)
+        assert ((got.cpu().double() - want).abs() <= tol).all()
+        assert torch.equal(got, ops.paged_attention_kv4(query, cache, tables, lens, 0.1, 6000))

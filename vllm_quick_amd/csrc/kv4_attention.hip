@@ -51,7 +51,9 @@ struct AttendArgs {
   uint32_t per_block_magic;  // ceil(2^32 / (block_size / 16)), or 0 for blocks of 16
   float scale;               // of the scores, times log2(e)
   int window, max_query_len;
-  int splits, chunk;  // pieces of a sequence, keys of one (the last piece takes what is left)
+  int splits;       // pieces that a sequence is cut into at most
+  int least;        // steps that a piece has at least, about,
+  float per_piece;  // and what share of the steps of all sequences together, but for a sequence's rounding
 };
 
 // Uniform integers that no kernel here writes, through the scalar cache: a vector load would return behind all the
@@ -384,8 +386,8 @@ struct Wave {
     load_values();
   }
 
-  // Runs over tiles first, first + stride, .. < last, the first of them loaded; all columns see all of the tiles that lie in whole_from ..
-  // whole_to - 1 of the keys.
+  // Runs over tiles first, first + stride, .. < last, the first of them loaded; all columns see all of the tiles that lie
+  // in whole_from .. whole_to - 1 of the keys.
   __device__ __forceinline__ void run(int first, int last, int stride, int length, int whole_from, int whole_to) {
     if (first >= last) return;
     int next = min(first + stride, last - 1);  // (the last step loads some tile again, which nobody looks at)
@@ -467,10 +469,49 @@ __device__ __forceinline__ Range range(const AttendArgs& a, const Sequence& s, i
   const int start = a.window > 0 ? max(0, whole_to - a.window) : 0;
   return Range{start / kTile, (end + kTile - 1) / kTile, a.window > 0 ? max(0, end - a.window) : 0, whole_to};
 }
-// How many pieces they come in: as many as a sequence of this length needs, at most `splits`.
-__device__ __forceinline__ int pieces_of(const AttendArgs& a, const Range& r) {
-  const int per_piece = a.chunk / kTile;
-  return max(1, min(a.splits, (r.last_tile - r.first_tile + per_piece - 1) / per_piece));
+// Steps of a piece: lengths are known here alone, and as many pieces as fill the chip should be about equal, whether one
+// long sequence has them all or each sequence has its own.
+__device__ __forceinline__ int keys_of(const AttendArgs& a, int b) {
+  const long long held = (long long)a.table_width * a.block_size, seen = (long long)a.window + a.max_query_len;
+  return max(0, (int)min((long long)a.seq_lens[b], a.window > 0 ? min(held, seen) : held));
+}
+__device__ __forceinline__ int steps_of_a_piece(const AttendArgs& a) {
+  float all = 0.f;
+#pragma unroll 4
+  for (int i = threadIdx.x & 63; i < a.seqs; i += 64) all += (float)keys_of(a, i);
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) all += __shfl_xor(all, m);
+  return __builtin_amdgcn_readfirstlane(max(a.least, (int)__builtin_ceilf(all * a.per_piece)));
+}
+// How many pieces a range of tiles comes in.
+__device__ __forceinline__ int pieces_of(const AttendArgs& a, int tiles, int steps) {
+  return max(1, min(a.splits, (tiles + steps / 2) / steps));
+}
+// Which piece of which sequence is the unit'th of all; b = seqs behind the last.
+__device__ __forceinline__ void find_piece(const AttendArgs& a, int unit, int steps, int& b, int& split) {
+  const int lane = threadIdx.x & 63;
+  int before = 0;
+  for (int first = 0; first < a.seqs; first += 64) {
+    int own = 0;
+    if (first + lane < a.seqs)  // (a window may begin and end inside a tile: two more)
+      own = pieces_of(a, keys_of(a, first + lane) / kTile + 2, steps);
+    int upto = own;
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) {
+      const int x = __shfl_up(upto, m);
+      upto += lane >= m ? x : 0;
+    }
+    const uint64_t beyond = __ballot(before + upto > unit);
+    if (beyond) {
+      const int at = __builtin_ctzll(beyond);
+      b = __builtin_amdgcn_readfirstlane(first + at);
+      split = unit - before - __builtin_amdgcn_readlane(upto - own, at);
+      return;
+    }
+    before += __builtin_amdgcn_readlane(upto, 63);
+  }
+  b = a.seqs;
+  split = 0;
 }
 
 // The rows of a sequence past max_query_len were promised not to exist: they say so.
@@ -491,26 +532,28 @@ __global__ void __launch_bounds__(64 * WAVES, NC == 1 ? 3 : 2) attend_split_kern
   __shared__ float part[WAVES][kCols][D + 4];
   __shared__ float maxima[WAVES][kCols], sums[WAVES][kCols];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int pair = blockIdx.x, b = pair / a.kv_heads, kv = pair - b * a.kv_heads;
-  const int split = blockIdx.y;
-  const int tile = gridDim.z - 1 - blockIdx.z;  // (those that see most come first)
-  const int per_piece = a.chunk / kTile;
+  const int unit = blockIdx.x / a.kv_heads, kv = blockIdx.x - unit * a.kv_heads;
+  const int tile = gridDim.y - 1 - blockIdx.y;  // (those that see most come first)
   Wave<T, D, NC, NC == 1> w(a);  // (16 columns are all there are)
-  // Without a window a piece begins where it does whatever the length, which is under way meanwhile: one round trip to
-  // memory less before the first keys.
-  // (Where most workgroups may find no queries to work on they ask first.)
-  const bool ahead = a.window == 0 && gridDim.z <= 2;
-  if (ahead) w.first_loads(b, kv, split * per_piece + wave, &part[wave][0][0]);
+  int b = unit, split = 0, steps = 0;
+  // Without a window the keys begin where they do whatever the length, which is under way meanwhile: one round trip to
+  // memory less before the first keys.  (Where most workgroups may find no queries to work on they ask first.)
+  const bool ahead = a.splits == 1 && a.window == 0 && gridDim.y <= 2;
+  if (__builtin_expect(a.splits > 1, 0)) {
+    steps = steps_of_a_piece(a);
+    find_piece(a, unit, steps, b, split);
+    if (b == a.seqs) return;
+  }
+  if (ahead) w.first_loads(b, kv, wave, &part[wave][0][0]);
   const Sequence s = sequence(a, b);
   const int queries = min(s.queries, a.max_query_len), cols = queries * a.group;
   if (tile == 0 && split == 0 && queries < s.queries) refuse_rows<T, D>(a, s, kv);
   const int col0 = tile * kCols;
   if (col0 >= cols) return;
   const Range r = range(a, s, col0, min(cols - 1, col0 + kCols - 1));
-  const int pieces = pieces_of(a, r);
+  const int tiles = r.last_tile - r.first_tile, pieces = a.splits == 1 ? 1 : pieces_of(a, tiles, steps);
   if (split >= pieces) return;
-  const int t0 = r.first_tile + split * per_piece + wave;
-  const int t1 = split == pieces - 1 ? r.last_tile : r.first_tile + (split + 1) * per_piece;
+  const int t0 = r.first_tile + tiles * split / pieces + wave, t1 = r.first_tile + tiles * (split + 1) / pieces;
   if (!ahead) w.first_loads(b, kv, t0, &part[wave][0][0]);
   w.begin(s, kv, col0, cols);
   w.run(t0, t1, WAVES, s.length, r.whole_from, r.whole_to);
@@ -583,7 +626,8 @@ __global__ void __launch_bounds__(256) attend_join_kernel(AttendArgs a) {
   if (qi < 0 || qi >= queries) return;  // a row of no sequence, or one past max_query_len: neither is written here
   const int cols = queries * a.group, col = qi * a.group + (at - row * a.heads) - kv * a.group;
   const int col0 = col / (16 * NC) * (16 * NC);
-  const int pieces = pieces_of(a, range(a, s, col0, min(cols - 1, col0 + 16 * NC - 1)));
+  const Range r = range(a, s, col0, min(cols - 1, col0 + 16 * NC - 1));
+  const int pieces = pieces_of(a, r.last_tile - r.first_tile, steps_of_a_piece(a));
   if (pieces == 1) return;  // written by the first kernel
   constexpr int kLanes = D / 4, kAtOnce = 64 / kLanes;
   const int lane = threadIdx.x & 63, part = lane / kLanes, d = 4 * (lane % kLanes);
@@ -677,7 +721,8 @@ __global__ void __launch_bounds__(256, 2) attend_prompt_kernel(AttendArgs a) {
 // How a call is laid over the chip, from its sizes alone.
 struct Plan {
   bool prompt;
-  int nc, tiles, waves, splits, chunk;
+  int nc, tiles, waves, splits, least, units;
+  float per_piece;
 };
 Plan plan(int tokens, int seqs, int heads, int kv_heads, int max_query_len, int max_seq_len, int window) {
   const long long group = heads / kv_heads, cols = max_query_len * group;
@@ -686,11 +731,14 @@ Plan plan(int tokens, int seqs, int heads, int kv_heads, int max_query_len, int 
   p.tiles = (int)((cols + 16 * p.nc - 1) / (16 * p.nc));
   p.waves = 4;
   p.splits = 1;
-  p.chunk = 1 << 27;
+  p.least = 1;
+  p.per_piece = 1.f;
+  p.units = seqs;
   // Column tiles that hold queries: of all rows together (a batch may mix one prompt with many single tokens), a tile a
   // sequence more where they do not fill their last.
-  const long long full = (tokens * group + 16 * p.nc - 1) / (16 * p.nc);
-  const long long most_tiles = (long long)seqs * p.tiles, tiles = full + seqs < most_tiles ? full + seqs : most_tiles;
+  const long long most_tiles = (long long)seqs * p.tiles;
+  const long long full = max_query_len == 1 ? most_tiles : (tokens * group + 16 * p.nc - 1) / (16 * p.nc);
+  const long long tiles = full + seqs < most_tiles ? full + seqs : most_tiles;
   // A wave for each column tile where these alone fill the chip, two waves a SIMD, and the rows are spread about evenly:
   // 2 x 8 kv heads x 1024 queries of 8 heads take 70 us so and 98 with waves that share the keys, 64 x 8 x 32 queries of
   // 4 heads over 1024 keys 60 and 71.  Below that some SIMDs idle while others have all the keys to run over: one
@@ -704,22 +752,30 @@ Plan plan(int tokens, int seqs, int heads, int kv_heads, int max_query_len, int 
   if (window > 0 && (long long)window + max_query_len < keys) keys = window + max_query_len;
   // Where a workgroup a CU is all there is, eight waves share up to 2048 keys and no second kernel runs: 16 x 4 kv heads
   // x 1029 keys of 64 take 11.8 us so, 14.6 with four waves and two pieces.  Otherwise as many pieces as fill the chip
-  // once (three workgroups of four waves a CU): 8 x 8 kv heads x 65536 keys of 128 take 90 us in 12 pieces, 104 in 24
-  // (the last round of workgroups leaves most CUs idle), 115 in 48.
+  // once (three workgroups of four waves a CU, two of 32 columns).
   if (groups * ((keys + 2047) / 2048) <= 256) p.waves = 8;
+  if (keys <= 512) return p;
   const long long least = p.waves == 8 ? 2048 : 512, most = (keys + least - 1) / least;
-  long long splits = (p.waves == 8 ? 256 : p.nc == 2 ? 512 : 768) / groups;
-  splits = splits < most ? splits : most;
-  splits = splits < 1 ? 1 : splits > 64 ? 64 : splits;
-  if (splits == 1) return p;
-  p.chunk = (int)(((keys + splits - 1) / splits + 127) / 128 * 128);
-  p.splits = (int)((keys + p.chunk - 1) / p.chunk);
+  long long cut = (p.waves == 8 ? 256 : p.nc == 2 ? 512 : 768) / groups;
+  cut = cut < 1 ? 1 : cut;
+  // A long sequence among short ones comes in more, at what looking for the pieces and a second kernel cost the others:
+  // 63 x 500 keys of 8 kv heads beside one of 65536 take 38 us so and 395 with a workgroup each, 64 lengths spread over
+  // their logarithm up to 32768 67 and 194, 64 x 4096 49 and 45.  Where sequences fill the chip several times over there
+  // is less to even out than that costs: 256 lengths of up to 16384 152 and 191, 256 x 2048 111 and 90.  (What is not
+  // taken up of a workspace costs nothing; it stays below 2^18 pieces of a query head.)
+  const long long room = (1LL << 18) / ((long long)tokens * heads);
+  long long splits = cut == 1 && groups > 1024 ? 1 : most < room ? most : room;
+  p.splits = (int)(splits < 1 ? 1 : splits > 64 ? 64 : splits);
+  p.least = (int)(least / kTile);
+  // (half a piece a sequence for the rounding of their numbers: one workgroup too many is a round too many)
+  p.per_piece = 1.f / ((float)kTile * (float)seqs * (cut == 1 ? 1.f : (float)cut - 0.5f));
+  // At most one piece a sequence more than its share, and 2 / 16 for the two tiles that are added to it.
+  p.units = p.splits > 1 ? (int)(seqs * (cut + 1) + (seqs + 3) / 4) : seqs;
   return p;
 }
 
 template <typename T, int D>
 int launch(const AttendArgs& a, const Plan& p, hipStream_t s) {
-  const unsigned pairs = (unsigned)a.seqs * (unsigned)a.kv_heads;
   if (p.prompt) {
     // the longest sequence first, and of each the columns that see most: the short ones fill the end.  In one order for
     // all, 2 x 2048 queries that see up to 2500 and 8192 keys leave 40 % of the CUs' time unused.  A kv head's workgroups
@@ -728,7 +784,7 @@ int launch(const AttendArgs& a, const Plan& p, hipStream_t s) {
     hipLaunchKernelGGL((attend_prompt_kernel<T, D, 2>), grid, dim3(256), 0, s, a);
     return serving_after_launch();
   }
-  const dim3 grid(pairs, (unsigned)p.splits, (unsigned)p.tiles);
+  const dim3 grid((unsigned)p.units * (unsigned)a.kv_heads, (unsigned)p.tiles);
   if (p.nc == 1 && p.waves == 4)
     hipLaunchKernelGGL((attend_split_kernel<T, D, 1, 4>), grid, dim3(256), 0, s, a);
   else if (p.nc == 1)
@@ -747,6 +803,10 @@ int launch(const AttendArgs& a, const Plan& p, hipStream_t s) {
   return serving_after_launch();
 }
 
+size_t workspace_of(const Plan& p, int tokens, int heads, int head_size) {
+  return p.splits == 1 ? 0 : (size_t)tokens * heads * p.splits * (head_size + 2) * sizeof(float);
+}
+
 bool sizes_ok(int tokens, int seqs, int heads, int kv_heads, int max_query_len, int max_seq_len, int window) {
   return tokens > 0 && seqs > 0 && heads > 0 && heads <= 65535 && kv_heads > 0 && kv_heads <= heads && heads % kv_heads == 0 &&
          max_query_len > 0 && max_seq_len > 0 && max_seq_len <= (1 << 27) && window >= 0;
@@ -758,7 +818,7 @@ extern "C" size_t serving_attend_kv4_workspace_bytes(int tokens, int seqs, int h
                                                      int max_query_len, int max_seq_len, int window) {
   if (!sizes_ok(tokens, seqs, heads, kv_heads, max_query_len, max_seq_len, window) || !head_size_ok(head_size)) return 0;
   const Plan p = plan(tokens, seqs, heads, kv_heads, max_query_len, max_seq_len, window);
-  return p.splits == 1 ? 0 : (size_t)tokens * heads * p.splits * (head_size + 2) * sizeof(float);
+  return workspace_of(p, tokens, heads, head_size);
 }
 
 extern "C" int serving_attend_kv4(const void* query, long long q_token, long long q_head, const void* cache,
@@ -780,7 +840,7 @@ extern "C" int serving_attend_kv4(const void* query, long long q_token, long lon
   if ((long long)seqs * kv_heads > 0x7fffffLL || (p.prompt && seqs > 65535) || p.tiles > (p.prompt ? 4 : 1) * 65535LL ||
       (long long)tokens * heads > (p.splits > 1 ? 0x3ffffffLL : 0x7fffffffLL))
     return SERVING_E_TOO_LARGE;
-  const size_t need = serving_attend_kv4_workspace_bytes(tokens, seqs, heads, kv_heads, head_size, max_query_len, max_seq_len, window);
+  const size_t need = workspace_of(p, tokens, heads, head_size);
   if (need && (!workspace || workspace_bytes < need)) return SERVING_E_WORKSPACE;
   if (need && !aligned16(workspace)) return SERVING_E_ALIGN;
   const int sixteens = block_size / 16;
@@ -788,7 +848,7 @@ extern "C" int serving_attend_kv4(const void* query, long long q_token, long lon
                static_cast<float*>(workspace), nullptr, table_width, tokens, seqs, heads, kv_heads, heads / kv_heads,
                (int)num_blocks, block_size,
                sixteens == 1 ? 0u : (uint32_t)(((1ULL << 32) + sixteens - 1) / sixteens),
-               scale * 1.44269504088896340736f, window, max_query_len, p.splits, p.chunk};
+               scale * 1.44269504088896340736f, window, max_query_len, p.splits, p.least, p.per_piece};
   if (need) a.part_ml = a.part_o + (size_t)tokens * heads * p.splits * head_size;
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (head_size == 64) return bf16_in ? launch<bf16, 64>(a, p, s) : launch<f16, 64>(a, p, s);
