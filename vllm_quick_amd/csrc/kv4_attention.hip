@@ -724,7 +724,7 @@ struct Plan {
   int nc, tiles, waves, splits, least, units;
   float per_piece;
 };
-Plan plan(int tokens, int seqs, int heads, int kv_heads, int max_query_len, int max_seq_len, int window) {
+Plan plan(int tokens, int seqs, int heads, int kv_heads, int max_query_len, int max_seq_len, int window, int head_size) {
   const long long group = heads / kv_heads, cols = max_query_len * group;
   Plan p;
   p.nc = cols > 16 ? 2 : 1;
@@ -750,21 +750,23 @@ Plan plan(int tokens, int seqs, int heads, int kv_heads, int max_query_len, int 
   const long long groups = tiles * kv_heads;
   long long keys = max_seq_len;
   if (window > 0 && (long long)window + max_query_len < keys) keys = window + max_query_len;
-  // Where a workgroup a CU is all there is, eight waves share up to 2048 keys and no second kernel runs: 16 x 4 kv heads
-  // x 1029 keys of 64 take 11.8 us so, 14.6 with four waves and two pieces.  Otherwise as many pieces as fill the chip
-  // once (three workgroups of four waves a CU, two of 32 columns).
+  // Where a workgroup a CU is all there is, eight waves share the keys, up to 2048 of them without a second kernel (16 x 4
+  // kv heads x 1029 keys of 64 take 11.8 us so, 14.6 with four waves and two pieces), more in pieces of 512 (8 kv heads x
+  // 4096 keys of 128 13.0 us; of 256 12.7, of 1024 14.7, of 2048 18.7; of 32 x 4096 14.7, 14.7, 15.5 and 19.3).
+  // Otherwise as many pieces as fill the chip once: four workgroups of four waves a CU, three for heads of 128, two of 32
+  // columns, which is what their registers allow (2 x 32 x 56000 keys of 64 60 us; in three or five a CU 63).
   if (groups * ((keys + 2047) / 2048) <= 256) p.waves = 8;
-  if (keys <= 512) return p;
-  const long long least = p.waves == 8 ? 2048 : 512, most = (keys + least - 1) / least;
-  long long cut = (p.waves == 8 ? 256 : p.nc == 2 ? 512 : 768) / groups;
+  if (keys <= (p.waves == 8 ? 2048 : 512)) return p;
+  const long long least = 512, most = (keys + least - 1) / least;
+  long long cut = (p.waves == 8 ? 256 : p.nc == 2 ? 512 : head_size == 64 ? 1024 : 768) / groups;
   cut = cut < 1 ? 1 : cut;
   // A long sequence among short ones comes in more, at what looking for the pieces and a second kernel cost the others:
   // 63 x 500 keys of 8 kv heads beside one of 65536 take 38 us so and 395 with a workgroup each, 64 lengths spread over
   // their logarithm up to 32768 67 and 194, 64 x 4096 49 and 45.  Where sequences fill the chip several times over there
-  // is less to even out than that costs: 256 lengths of up to 16384 152 and 191, 256 x 2048 111 and 90.  (What is not
+  // is less to even out than that costs, and so where the longest are short: 256 lengths of up to 16384 152 and 191, 256 x 2048 111 and 90.  (What is not
   // taken up of a workspace costs nothing; it stays below 2^18 pieces of a query head.)
   const long long room = (1LL << 18) / ((long long)tokens * heads);
-  long long splits = cut == 1 && groups > 1024 ? 1 : most < room ? most : room;
+  long long splits = cut == 1 && (groups > 1024 || keys <= 2048) ? 1 : most < room ? most : room;
   p.splits = (int)(splits < 1 ? 1 : splits > 64 ? 64 : splits);
   p.least = (int)(least / kTile);
   // (half a piece a sequence for the rounding of their numbers: one workgroup too many is a round too many)
@@ -817,7 +819,7 @@ bool sizes_ok(int tokens, int seqs, int heads, int kv_heads, int max_query_len, 
 extern "C" size_t serving_attend_kv4_workspace_bytes(int tokens, int seqs, int heads, int kv_heads, int head_size,
                                                      int max_query_len, int max_seq_len, int window) {
   if (!sizes_ok(tokens, seqs, heads, kv_heads, max_query_len, max_seq_len, window) || !head_size_ok(head_size)) return 0;
-  const Plan p = plan(tokens, seqs, heads, kv_heads, max_query_len, max_seq_len, window);
+  const Plan p = plan(tokens, seqs, heads, kv_heads, max_query_len, max_seq_len, window, head_size);
   return workspace_of(p, tokens, heads, head_size);
 }
 
@@ -836,7 +838,7 @@ extern "C" int serving_attend_kv4(const void* query, long long q_token, long lon
     return SERVING_E_SHAPE;
   if ((long long)table_width * block_size > (1LL << 27)) return SERVING_E_TOO_LARGE;
   if (!aligned16(query) || !aligned16(cache) || !aligned16(out) || q_token % 8 || q_head % 8) return SERVING_E_ALIGN;
-  const Plan p = plan(tokens, seqs, heads, kv_heads, max_query_len, max_seq_len, window);
+  const Plan p = plan(tokens, seqs, heads, kv_heads, max_query_len, max_seq_len, window, head_size);
   if ((long long)seqs * kv_heads > 0x7fffffLL || (p.prompt && seqs > 65535) || p.tiles > (p.prompt ? 4 : 1) * 65535LL ||
       (long long)tokens * heads > (p.splits > 1 ? 0x3ffffffLL : 0x7fffffffLL))
     return SERVING_E_TOO_LARGE;
