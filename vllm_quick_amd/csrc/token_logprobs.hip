@@ -394,7 +394,7 @@ __global__ void __launch_bounds__(256) join_kernel(Args a, int rows) {
 // A lane holds 32 elements; the first 16 bytes of a segment may hold 7 (3) elements in front of it.  A workgroup of
 // 1024 lanes takes a row of up to 32760 tokens alone, which is one launch instead of two; where there are enough rows to
 // fill the chip, segments of 256 lanes do more, since a CU runs several (one loads while another sums): 4096 x 32000 fp32
-// 116 us against 222.
+// with 20 alternatives 105 us against 154, 1836 x 10580 bf16 24 against 52.
 struct Plan {
   int threads, segments, segment;
 };
