@@ -218,3 +218,23 @@ def test_a_captured_step_of_sequences_that_grow(ops, cuda):
         want, tol = orc.attend(case[0], case[1], case[2], torch.tensor(now), case[4], 0.1, 0, True)
         assert ((got.cpu().double() - want).abs() <= tol).all()
         assert torch.equal(got, ops.paged_attention_kv4(query, cache, tables, lens, 0.1, 6000))
+
+
+def test_what_is_written_counts_as_changed(ops, cuda):
+    """A tensor saved for a backward pass and then written to here is found out, as after torch's own writes in place."""
+    query, cache, tables, lens, start = [x.to(cuda) for x in attend_case([30, 4], [1, 1], 4, 2, 64, 16, torch.float16, 107)]
+    slots = torch.tensor([-1, -1], device=cuda)
+    new = torch.zeros(2, 2, 64, dtype=torch.float16, device=cuda)
+    before = cache._version
+    ops.rope_append_kv4(slots, query, new, new, torch.zeros(1, 64, device=cuda), cache, slots)
+    assert cache._version > before
+    leaf = torch.ones(2, 4, 64, dtype=torch.float16, device=cuda, requires_grad=True)
+    out = torch.zeros_like(query)
+    loss = (leaf * out).sum()
+    ops.paged_attention_kv4(query, cache, tables, lens, 0.1, 30, out=out)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with torch.inference_mode():
+        inner = torch.zeros_like(query)
+    ops.paged_attention_kv4(query, cache, tables, lens, 0.1, 30, out=inner)
+    assert torch.equal(inner, out)

@@ -444,7 +444,7 @@ struct Wave {
     keeps = true;
   }
 
-  // Element d of the result of this lane's column, as sums of p v 2^weight_log: out(piece of kEach elements, first element, values).
+  // Element d of the result of this lane's column, as sums of p v 2^weight_log: out(first of kEach elements, values).
   template <typename F>
   __device__ __forceinline__ void results(int n, F&& out) {
     constexpr int kEach = kRows;  // neighbouring elements that a lane holds: element kEach (4 g + r) + m
@@ -763,8 +763,9 @@ Plan plan(int tokens, int seqs, int heads, int kv_heads, int max_query_len, int 
   // A long sequence among short ones comes in more, at what looking for the pieces and a second kernel cost the others:
   // 63 x 500 keys of 8 kv heads beside one of 65536 take 38 us so and 395 with a workgroup each, 64 lengths spread over
   // their logarithm up to 32768 67 and 194, 64 x 4096 49 and 45.  Where sequences fill the chip several times over there
-  // is less to even out than that costs, and so where the longest are short: 256 lengths of up to 16384 152 and 191, 256 x 2048 111 and 90.  (What is not
-  // taken up of a workspace costs nothing; it stays below 2^18 pieces of a query head.)
+  // is less to even out than that costs, and so where the longest are short: 256 lengths of up to 16384 152 and 191,
+  // 256 x 2048 111 and 90, 127 x 800 35 and 25.  (What is not taken up of a workspace costs nothing; it stays below 2^18
+  // pieces of a query head.)
   const long long room = (1LL << 18) / ((long long)tokens * heads);
   long long splits = cut == 1 && (groups > 1024 || keys <= 2048) ? 1 : most < room ? most : room;
   p.splits = (int)(splits < 1 ? 1 : splits > 64 ? 64 : splits);

@@ -73,6 +73,11 @@ void no_gradient(const Tensor& t, const char* what, const char* name) {
               " requires a gradient, which this operator does not give: call it under torch.no_grad() or on a detached tensor");
 }
 
+// What a call writes into counts as changed in place for whoever saved it for a backward pass.
+void written(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // Rows of heads whose elements lie together, at addresses and strides that 16-byte loads can take.
 Tensor heads_of(const Tensor& t) {
   const bool fits = t.stride(2) == 1 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 &&
@@ -134,6 +139,7 @@ Tensor rope_append_kv4(const Tensor& positions, const Tensor& query, const Tenso
                                     cos_sin.size(0), cache.size(0), (int)block_size, bf16,
                                     getCurrentHIPStreamMasqueradingAsCUDA().stream()),
             what);
+  written(cache);
   return out;
 }
 
@@ -217,6 +223,7 @@ Tensor paged_attention_kv4(const Tensor& query, const Tensor& cache, const Tenso
                                (int)max_query_len, (int)max_seq_len, bf16, bytes ? workspace.data_ptr() : nullptr, bytes,
                                getCurrentHIPStreamMasqueradingAsCUDA().stream()),
             what);
+  if (out_) written(out);
   return out;
 }
 
