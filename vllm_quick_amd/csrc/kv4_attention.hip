@@ -841,7 +841,7 @@ extern "C" int serving_attend_kv4(const void* query, long long q_token, long lon
   if (!aligned16(query) || !aligned16(cache) || !aligned16(out) || q_token % 8 || q_head % 8) return SERVING_E_ALIGN;
   const Plan p = plan(tokens, seqs, heads, kv_heads, max_query_len, max_seq_len, window, head_size);
   if ((long long)seqs * kv_heads > 0x7fffffLL || (p.prompt && seqs > 65535) || p.tiles > (p.prompt ? 4 : 1) * 65535LL ||
-      (long long)tokens * heads > (p.splits > 1 ? 0x3ffffffLL : 0x7fffffffLL))
+      (long long)tokens * heads > 0x7fffffffLL)
     return SERVING_E_TOO_LARGE;
   const size_t need = workspace_of(p, tokens, heads, head_size);
   if (need && (!workspace || workspace_bytes < need)) return SERVING_E_WORKSPACE;
