@@ -141,3 +141,22 @@ def test_more_than_2_31_logits(ops, cuda):
 def test_empty(ops, cuda):
     out = ops.token_logprobs(torch.zeros(0, 10, device=cuda), torch.zeros(0, dtype=torch.int64, device=cuda), 3)
     assert [tuple(t.shape) for t in out] == [(0, ), (0, ), (0, 3), (0, 3)]
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
+@pytest.mark.parametrize("rows,vocab,top", [
+    (2, 12000, 64), (3, 16377, 5), (2, 16378, 20), (2, 16381, 3), (2, 16382, 1), (2, 16384, 2), (2, 16385, 64), (300, 9000, 4),
+    (1030, 8500, 2),  # too many rows for one workgroup each
+])
+def test_logprobs_of_middling_vocabularies(ops, cuda, rows, vocab, top, dtype):
+    check(ops, cuda, *random_logits(rows, vocab, TYPES[dtype], rows * 3 + vocab), top)
+
+
+@pytest.mark.parametrize("top", [1, 64])
+def test_rows_of_equals_of_a_middling_vocabulary(ops, cuda, top):
+    x = torch.zeros(4, 14001)
+    x[1, 1::3] = 1.0
+    x[2] = torch.arange(14001).float().div(400, rounding_mode="floor")
+    x[3, 17] = float("nan")
+    for dtype in TYPES.values():
+        check(ops, cuda, x.to(dtype), torch.full((4, ), 14000), top)

@@ -20,7 +20,7 @@ using namespace serving;
 constexpr int kMaxTop = 64;       // groups that are ranked for the bound
 constexpr int kCandidates = 1024;  // elements not below the bound that LDS takes; more (rows of equals) go the long way
 
-constexpr int kFewRows = 256;  // a workgroup of 1024 lanes for each CU
+constexpr int kFewRows = 256;  // a workgroup of 1024 lanes for each CU, or four of 512
 constexpr int kMaxVocab = 64 * 32760;  // 64 segments: a lane of the join each, and their keys in LDS
 
 typedef unsigned long long u64;
@@ -392,16 +392,23 @@ __global__ void __launch_bounds__(256) join_kernel(Args a, int rows) {
 }
 
 // A lane holds 32 elements; the first 16 bytes of a segment may hold 7 (3) elements in front of it.  A workgroup of
-// 1024 lanes takes a row of up to 32760 tokens alone, which is one launch instead of two; where there are enough rows to
-// fill the chip, segments of 256 lanes do more, since a CU runs several (one loads while another sums): 4096 x 32000 fp32
-// with 20 alternatives 105 us against 154, 1836 x 10580 bf16 24 against 52.
+// 1024 lanes takes a row of up to 32760 tokens alone, one of 512 half of that, which is one launch instead of two; where
+// there are enough rows to fill the chip, segments of 256 lanes do more, since a CU runs several (one loads while another
+// sums): 4096 x 32000 fp32 with 20 alternatives 105 us against 154, 4096 x 16000 bf16 56 against 61 with 512 lanes; but
+// 300 x 9000 bf16 11.1 against 9.2, 200 x 30000 12.1 against 8.7 with 1024.
 struct Plan {
   int threads, segments, segment;
 };
 Plan plan(int rows, int vocab, int type) {
   const int spare = type == 2 ? 3 : 7;
   Plan p;
-  p.threads = vocab > 16 * (256 * 32 - 8) || (vocab + spare > 256 * 32 && vocab + spare <= 1024 * 32 && rows <= kFewRows) ? 1024 : 256;
+  p.threads = 256;
+  if (vocab + spare > 256 * 32) {
+    if (vocab + spare <= 512 * 32 && rows <= 4 * kFewRows)
+      p.threads = 512;
+    else if (vocab > 16 * (256 * 32 - 8) || (vocab + spare <= 1024 * 32 && rows <= kFewRows))
+      p.threads = 1024;
+  }
   const int most = p.threads * 32 - 8;
   if (vocab + spare <= p.threads * 32) {
     p.segments = 1, p.segment = vocab;
@@ -419,6 +426,8 @@ int launch(const Args& a, int rows, int threads, hipStream_t s) {
   const dim3 grid((unsigned)rows * (unsigned)a.segments);
   if (threads == 256)
     hipLaunchKernelGGL((logprobs_kernel<TYPE, 256, kAll>), grid, dim3(256), 0, s, a);
+  else if (threads == 512)
+    hipLaunchKernelGGL((logprobs_kernel<TYPE, 512, kAll>), grid, dim3(512), 0, s, a);
   else
     hipLaunchKernelGGL((logprobs_kernel<TYPE, 1024, kAll>), grid, dim3(1024), 0, s, a);
   if (a.segments > 1) {
