@@ -238,3 +238,37 @@ def test_what_is_written_counts_as_changed(ops, cuda):
         inner = torch.zeros_like(query)
     ops.paged_attention_kv4(query, cache, tables, lens, 0.1, 30, out=inner)
     assert torch.equal(inner, out)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("counts,large", [([1, 1], False), ([3, 40], False), ([20, 40], True)])
+def test_blocks_that_a_window_has_left_behind_may_hold_anything(ops, cuda, counts, large, dtype):
+    """Freed blocks in front of a window: parameters of infinity or NaN, and ids that no cache has, change nothing."""
+    window, p, d = 40, 16, 64
+    query, cache, tables, lens, start = attend_case([100, 333], counts, 4, 2, d, p, TYPES[dtype], 109, gain=1500.0)
+    if large:
+        query, cache, tables, lens, start = in_a_large_batch((query, cache, tables, lens, start), 2048)
+    run = lambda c, t: ops.paged_attention_kv4(query.to(cuda), c.to(cuda), t.to(cuda), lens.to(cuda), 0.125 / 1500, 333,  # noqa: E731
+                                               query_start=start.to(cuda), max_query_len=max(counts), window=window).cpu()
+    rows = sum(counts)
+    want, tol = orc.attend(query, cache, tables, lens, start, 0.125 / 1500, window, dtype == "fp16")
+    assert bool(torch.isfinite(want[:rows]).all())
+    for bits in (0x7c00, 0x7e00, 0xfc00):
+        wrong, left = cache.clone(), tables.clone()
+        for b in range(2):
+            first = int(lens[b]) - counts[b] + 1 - window  # the first key that the first row sees
+            for page in range(first // p):
+                wrong[tables[b, page].long()].view(torch.int16)[:, p * d // 2:] = bits - (1 << 16 if bits > 0x7fff else 0)
+        for gone in (False, True):
+            if gone:
+                wrong[0] = 0
+                spare = [i for i in range(cache.shape[0]) if i not in tables.flatten().tolist()]
+                if 0 not in spare:  # block 0 is one of a sequence's: leave it to the others to be read in its place
+                    wrong[0] = cache[0]
+                else:
+                    wrong[0].view(torch.int16)[:, p * d // 2:] = bits - (1 << 16 if bits > 0x7fff else 0)
+                for b in range(2):
+                    left[b, :(int(lens[b]) - counts[b] + 1 - window) // p] = -1
+            got = run(wrong, left)[:rows].double()
+            off = int((~((got - want[:rows]).abs() <= tol[:rows])).sum())
+            assert off == 0, (hex(bits), gone, off)

@@ -111,6 +111,7 @@ struct Wave {
   f16x8 q[NC][kSteps];
   float qs[NC];          // sum of the query, in the unit of the scores
   int lim[NC], low[NC];  // keys that a column sees: low .. lim - 1
+  int least_low;         // of all columns of the wave
   float shift[NC];       // p 2^weight_log = 2^(score + shift): no p passes 2^kSlack
   float sum[NC], flat[NC];
   float unit_score;      // what makes a score (in powers of two) of a product
@@ -148,6 +149,7 @@ struct Wave {
   // The queries.
   __device__ __forceinline__ void begin(const Sequence& s, int kv, int col0, int cols) {
     last_page = max(0, page_of((s.length - 1) >> 4));
+    least_low = a.window > 0 ? max(0, s.before + col0 / a.group + 1 - a.window) : 0;
     vref = 0x1p-40f;
     weight_log = kWeightLog + 40.f;
     float x[NC][kSteps][8], big = 0.f;
@@ -334,10 +336,12 @@ struct Wave {
       }
     }
     load_keys();
-    if (MASK) {  // parameters behind the sequence may be anything
+    if (MASK) {  // parameters behind the sequence, before every window and of unknown blocks may be anything
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (from + 16 * (i / 4) + 4 * g + i % 4 >= length) vp[i / 4][i % 4] = 0;
+      for (int i = 0; i < 8; ++i) {
+        const int key = from + 16 * (i / 4) + 4 * g + i % 4;
+        if (key >= length || key < least_low || !known_now[i / 4]) vp[i / 4][i % 4] = 0;
+      }
     }
     f16x2 big = as_pair(vp[0][0]);
 #pragma unroll
