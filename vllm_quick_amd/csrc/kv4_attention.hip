@@ -540,7 +540,7 @@ __global__ void __launch_bounds__(64 * WAVES, NC == 1 ? 3 : 2) attend_split_kern
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int unit = blockIdx.x / a.kv_heads, kv = blockIdx.x - unit * a.kv_heads;
   const int tile = gridDim.y - 1 - blockIdx.y;  // (those that see most come first)
-  Wave<T, D, NC, NC == 1> w(a);  // (16 columns are all there are)
+  Wave<T, D, NC, NC == 1> w(a);  // (16 columns are all there are, or all that is small)
   int b = unit, split = 0, steps = 0;
   // Without a window the keys begin where they do whatever the length, which is under way meanwhile: one round trip to
   // memory less before the first keys.  (Where most workgroups may find no queries to work on they ask first.)
@@ -736,18 +736,22 @@ struct Plan {
 Plan plan(int tokens, int seqs, int heads, int kv_heads, int max_query_len, int max_seq_len, int window, int head_size) {
   const long long group = heads / kv_heads, cols = max_query_len * group;
   Plan p;
-  p.nc = cols > 16 ? 2 : 1;
-  p.tiles = (int)((cols + 16 * p.nc - 1) / (16 * p.nc));
   p.waves = 4;
   p.splits = 1;
   p.least = 1;
   p.per_piece = 1.f;
   p.units = seqs;
-  // Column tiles that hold queries: of all rows together (a batch may mix one prompt with many single tokens), a tile a
-  // sequence more where they do not fill their last.
-  const long long most_tiles = (long long)seqs * p.tiles;
-  const long long full = max_query_len == 1 ? most_tiles : (tokens * group + 16 * p.nc - 1) / (16 * p.nc);
-  const long long tiles = full + seqs < most_tiles ? full + seqs : most_tiles;
+  // Column tiles of nc x 16, and those of them that hold queries: of all rows together (a batch may mix one prompt with
+  // many single tokens), a tile a sequence more where they do not fill their last.
+  long long most_tiles, full, groups;
+  const auto tile = [&](int nc) {
+    p.nc = nc;
+    p.tiles = (int)((cols + 16 * nc - 1) / (16 * nc));
+    most_tiles = (long long)seqs * p.tiles;
+    full = max_query_len == 1 ? most_tiles : (tokens * group + 16 * nc - 1) / (16 * nc);
+    groups = (full + seqs < most_tiles ? full + seqs : most_tiles) * kv_heads;
+  };
+  tile(cols > 16 ? 2 : 1);
   // A wave for each column tile where these alone fill the chip, two waves a SIMD, and the rows are spread about evenly:
   // 2 x 8 kv heads x 1024 queries of 8 heads take 70 us so and 98 with waves that share the keys, 64 x 8 x 32 queries of
   // 4 heads over 1024 keys 60 and 71.  Below that some SIMDs idle while others have all the keys to run over: one
@@ -756,15 +760,22 @@ Plan plan(int tokens, int seqs, int heads, int kv_heads, int max_query_len, int 
   // (2048 queries of 8 x 4 heads over 65536 keys, one round: 2970 and 2710; twice 2048 over 8192, two: 633 and 630).
   p.prompt = cols > 64 && full * kv_heads >= (max_seq_len > 2048 ? 4096 : 2048) && 2 * full >= most_tiles;
   if (p.prompt) return p;
-  const long long groups = tiles * kv_heads;
   long long keys = max_seq_len;
   if (window > 0 && (long long)window + max_query_len < keys) keys = window + max_query_len;
-  // Where a workgroup a CU is all there is, eight waves share the keys, up to 2048 of them without a second kernel (16 x 4
+  // Where a workgroup a CU is all there is eight waves share the keys, up to 2048 of them without a second kernel (16 x 4
   // kv heads x 1029 keys of 64 take 11.8 us so, 14.6 with four waves and two pieces), more in pieces of 512 (8 kv heads x
   // 4096 keys of 128 13.0 us; of 256 12.7, of 1024 14.7, of 2048 18.7; of 32 x 4096 14.7, 14.7, 15.5 and 19.3).
   // Otherwise as many pieces as fill the chip once: four workgroups of four waves a CU, three for heads of 128, two of 32
   // columns, which is what their registers allow (2 x 32 x 56000 keys of 64 60 us; in three or five a CU 63).
-  if (groups * ((keys + 2047) / 2048) <= 256) p.waves = 8;
+  const long long rounds = (keys + 2047) / 2048;
+  if (p.nc == 2 && groups * rounds <= 256) {
+    // ... and tiles of 16 columns spread the work wider where they fit too: 16 x 4 kv heads x 5 queries of 7 heads over 1024
+    // keys of 64 9.0 us against 11.9, one query of 128 heads over 2000 keys of 128 14.4 against 19.4; of half as many
+    // again no more (8 x 8 x 64 columns over 4096 keys 39.8 and 38.1).
+    tile(1);
+    if (groups * rounds > 256) tile(2);
+  }
+  if (groups * rounds <= 256) p.waves = 8;
   if (keys <= (p.waves == 8 ? 2048 : 512)) return p;
   const long long least = 512, most = (keys + least - 1) / least;
   long long cut = (p.waves == 8 ? 256 : p.nc == 2 ? 512 : head_size == 64 ? 1024 : 768) / groups;
