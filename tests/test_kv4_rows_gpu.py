@@ -272,3 +272,17 @@ def test_blocks_that_a_window_has_left_behind_may_hold_anything(ops, cuda, count
             got = run(wrong, left)[:rows].double()
             off = int((~((got - want[:rows]).abs() <= tol[:rows])).sum())
             assert off == 0, (hex(bits), gone, off)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("seqs,kv,d,window", [
+    (200, 4, 128, 0), (200, 4, 128, 30),    # two waves a workgroup
+    (260, 4, 64, 0), (400, 4, 128, 0),      # one and two
+    (530, 4, 64, 0), (530, 4, 64, 7),       # one
+    (1600, 1, 128, 0),
+])
+def test_many_short_sequences(ops, cuda, seqs, kv, d, window, dtype):
+    lens = [(11 * i) % 140 for i in range(seqs)]
+    case = attend_case(lens, [1] * seqs, kv, kv, d, 16, TYPES[dtype], seqs)
+    check_attend(ops, cuda, case, window=window, ragged=False)
+    check_attend(ops, cuda, case, window=window, ragged=False, max_seq_len=1)  # (the rest of them is read all the same)

@@ -776,9 +776,13 @@ Plan plan(int tokens, int seqs, int heads, int kv_heads, int max_query_len, int 
     if (groups * rounds > 256) tile(2);
   }
   if (groups * rounds <= 256) p.waves = 8;
+  const long long fill = p.nc == 2 ? 512 : head_size == 64 ? 1024 : 768;
+  // More short sequences than fill the chip once take fewer waves each, so that it holds more of them: 1024 x 250 keys of
+  // 128 10.4 us with two waves, 13.7 with four, 11.7 with one; 2048 x 129 16.9, 21.5 and 12.6, x 500 30.2, 31.3 and 25.0.
+  if (keys <= 512 && p.nc == 1 && groups > fill) p.waves = groups > 2 * fill ? 1 : 2;
   if (keys <= (p.waves == 8 ? 2048 : 512)) return p;
   const long long least = 512, most = (keys + least - 1) / least;
-  long long cut = (p.waves == 8 ? 256 : p.nc == 2 ? 512 : head_size == 64 ? 1024 : 768) / groups;
+  long long cut = (p.waves == 8 ? 256 : fill) / groups;
   cut = cut < 1 ? 1 : cut;
   // A long sequence among short ones comes in more, at what looking for the pieces and a second kernel cost the others:
   // 63 x 500 keys of 8 kv heads beside one of 65536 take 38 us so and 395 with a workgroup each, 64 lengths spread over
@@ -808,7 +812,11 @@ int launch(const AttendArgs& a, const Plan& p, hipStream_t s) {
     return serving_after_launch();
   }
   const dim3 grid((unsigned)p.units * (unsigned)a.kv_heads, (unsigned)p.tiles);
-  if (p.nc == 1 && p.waves == 4)
+  if (p.nc == 1 && p.waves == 1)
+    hipLaunchKernelGGL((attend_split_kernel<T, D, 1, 1>), grid, dim3(64), 0, s, a);
+  else if (p.nc == 1 && p.waves == 2)
+    hipLaunchKernelGGL((attend_split_kernel<T, D, 1, 2>), grid, dim3(128), 0, s, a);
+  else if (p.nc == 1 && p.waves == 4)
     hipLaunchKernelGGL((attend_split_kernel<T, D, 1, 4>), grid, dim3(256), 0, s, a);
   else if (p.nc == 1)
     hipLaunchKernelGGL((attend_split_kernel<T, D, 1, 8>), grid, dim3(512), 0, s, a);
