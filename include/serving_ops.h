@@ -87,7 +87,7 @@ int serving_read_kv4(const void* cache, const int64_t* slots, void* key, void* v
 /*
  * out[t] [tokens, heads, D] = softmax(scale * query[t] . keys) values over the cache.
  * Sequence b (of seqs) has seq_lens[b] tokens in the cache, in the blocks tables[b * table_stride + i], i = 0, 1, ..
- * (at most table_width of them), and the query rows query_start[b] .. query_start[b + 1] - 1, which are its LAST
+ * (at most table_width of them), and the query rows query_start[b] .. query_start[b + 1] - 1 (ascending), which are its LAST
  * tokens: row i of n sees keys 0 .. seq_lens[b] - n + i, with window > 0 only the last `window` of these.
  * query_start NULL: one row for each sequence (tokens = seqs).  heads is a multiple of kv_heads; query head h reads
  * kv head h / (heads / kv_heads).  A row that sees no key gives zeros; rows of no sequence are left as they were; rows

@@ -51,6 +51,7 @@ struct AttendArgs {
   uint32_t per_block_magic;  // ceil(2^32 / (block_size / 16)), or 0 for blocks of 16
   float scale;               // of the scores, times log2(e)
   int window, max_query_len;
+  int search;       // whether workgroups are numbered through all sequences, or each sequence has `tiles` of them
   int splits;       // pieces that a sequence is cut into at most
   int least;        // steps that a piece has at least, about,
   float per_piece;  // and what share of the steps of all sequences together, but for a sequence's rounding
@@ -479,26 +480,44 @@ __device__ __forceinline__ int keys_of(const AttendArgs& a, int b) {
   const long long held = (long long)a.table_width * a.block_size, seen = (long long)a.window + a.max_query_len;
   return max(0, (int)min((long long)a.seq_lens[b], a.window > 0 ? min(held, seen) : held));
 }
+template <int NC>
+__device__ __forceinline__ int tiles_of(const AttendArgs& a, int b) {
+  int queries = 1;
+  if (a.query_start) {
+    int row = a.query_start[b];
+    queries = a.query_start[b + 1] - row;
+    if (row < 0 || row > a.tokens) row = a.tokens;
+    queries = min(max(0, min(queries, a.tokens - row)), a.max_query_len);
+  }
+  return (queries * a.group + 16 * NC - 1) / (16 * NC);
+}
+template <int NC>
 __device__ __forceinline__ int steps_of_a_piece(const AttendArgs& a) {
   float all = 0.f;
 #pragma unroll 4
-  for (int i = threadIdx.x & 63; i < a.seqs; i += 64) all += (float)keys_of(a, i);
+  for (int i = threadIdx.x & 63; i < a.seqs; i += 64) all += (float)keys_of(a, i) * (float)tiles_of<NC>(a, i);
 #pragma unroll
   for (int m = 1; m < 64; m <<= 1) all += __shfl_xor(all, m);
   return __builtin_amdgcn_readfirstlane(max(a.least, (int)__builtin_ceilf(all * a.per_piece)));
 }
-// How many pieces a range of tiles comes in.
-__device__ __forceinline__ int pieces_of(const AttendArgs& a, int tiles, int steps) {
-  return max(1, min(a.splits, (tiles + steps / 2) / steps));
+// How many pieces a range of steps comes in (5/8: equal sequences, whose share is their number less a half, come in just
+// that number).
+__device__ __forceinline__ int pieces_of(const AttendArgs& a, int range, int steps) {
+  return max(1, min(a.splits, (range + 5 * steps / 8) / steps));
 }
-// Which piece of which sequence is the unit'th of all; b = seqs behind the last.
-__device__ __forceinline__ void find_piece(const AttendArgs& a, int unit, int steps, int& b, int& split) {
+// Which column tile and piece of which sequence is the unit'th of all; b = seqs behind the last.  The workgroups that
+// have no work are so the last: between others they would keep CUs from these, since workgroups go to the CUs in turn
+// (512 queries of 8 x 4 heads over 8192 keys 97 us, 186 with one for nothing beside each).
+template <int NC>
+__device__ __forceinline__ void find_piece(const AttendArgs& a, int unit, int steps, int& b, int& tile, int& split) {
   const int lane = threadIdx.x & 63;
   int before = 0;
   for (int first = 0; first < a.seqs; first += 64) {
-    int own = 0;
-    if (first + lane < a.seqs)  // (a window may begin and end inside a tile: two more)
-      own = pieces_of(a, keys_of(a, first + lane) / kTile + 2, steps);
+    int pieces = 0, own = 0;
+    if (first + lane < a.seqs) {  // (a window may begin and end inside a step: two more)
+      pieces = a.splits == 1 ? 1 : pieces_of(a, keys_of(a, first + lane) / kTile + 2, steps);
+      own = pieces * tiles_of<NC>(a, first + lane);
+    }
     int upto = own;
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) {
@@ -509,13 +528,16 @@ __device__ __forceinline__ void find_piece(const AttendArgs& a, int unit, int st
     if (beyond) {
       const int at = __builtin_ctzll(beyond);
       b = __builtin_amdgcn_readfirstlane(first + at);
-      split = unit - before - __builtin_amdgcn_readlane(upto - own, at);
+      const int left = before + __builtin_amdgcn_readlane(upto, at) - 1 - unit;  // (tiles that see most come first)
+      pieces = __builtin_amdgcn_readlane(pieces, at);
+      tile = left / pieces;
+      split = left - tile * pieces;
       return;
     }
     before += __builtin_amdgcn_readlane(upto, 63);
   }
   b = a.seqs;
-  split = 0;
+  tile = split = 0;
 }
 
 // The rows of a sequence past max_query_len were promised not to exist: they say so.
@@ -539,15 +561,14 @@ __global__ void __launch_bounds__(64 * WAVES, NC == 1 ? 3 : 2) attend_split_kern
   __shared__ float maxima[WAVES][kCols], sums[WAVES][kCols];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int unit = blockIdx.x / a.kv_heads, kv = blockIdx.x - unit * a.kv_heads;
-  const int tile = gridDim.y - 1 - blockIdx.y;  // (those that see most come first)
   Wave<T, D, NC, NC == 1> w(a);  // (16 columns are all there are, or all that is small)
-  int b = unit, split = 0, steps = 0;
+  int b = unit, tile = gridDim.y - 1 - blockIdx.y, split = 0, steps = 1;  // (tiles that see most come first)
   // Without a window the keys begin where they do whatever the length, which is under way meanwhile: one round trip to
-  // memory less before the first keys.  (Where most workgroups may find no queries to work on they ask first.)
-  const bool ahead = a.splits == 1 && a.window == 0 && gridDim.y <= 2;
-  if (__builtin_expect(a.splits > 1, 0)) {
-    steps = steps_of_a_piece(a);
-    find_piece(a, unit, steps, b, split);
+  // memory less before the first keys.
+  const bool ahead = a.window == 0 && !a.search;  // (few tiles are without queries then)
+  if (__builtin_expect(a.search, 0)) {
+    if (a.splits > 1) steps = steps_of_a_piece<NC>(a);
+    find_piece<NC>(a, unit, steps, b, tile, split);
     if (b == a.seqs) return;
   }
   if (ahead) w.first_loads(b, kv, wave, &part[wave][0][0]);
@@ -557,9 +578,9 @@ __global__ void __launch_bounds__(64 * WAVES, NC == 1 ? 3 : 2) attend_split_kern
   const int col0 = tile * kCols;
   if (col0 >= cols) return;
   const Range r = range(a, s, col0, min(cols - 1, col0 + kCols - 1));
-  const int tiles = r.last_tile - r.first_tile, pieces = a.splits == 1 ? 1 : pieces_of(a, tiles, steps);
+  const int all = r.last_tile - r.first_tile, pieces = a.splits == 1 ? 1 : pieces_of(a, all, steps);
   if (split >= pieces) return;
-  const int t0 = r.first_tile + tiles * split / pieces + wave, t1 = r.first_tile + tiles * (split + 1) / pieces;
+  const int t0 = r.first_tile + all * split / pieces + wave, t1 = r.first_tile + all * (split + 1) / pieces;
   if (!ahead) w.first_loads(b, kv, t0, &part[wave][0][0]);
   w.begin(s, kv, col0, cols);
   w.run(t0, t1, WAVES, s.length, r.whole_from, r.whole_to);
@@ -633,7 +654,7 @@ __global__ void __launch_bounds__(256) attend_join_kernel(AttendArgs a) {
   const int cols = queries * a.group, col = qi * a.group + (at - row * a.heads) - kv * a.group;
   const int col0 = col / (16 * NC) * (16 * NC);
   const Range r = range(a, s, col0, min(cols - 1, col0 + 16 * NC - 1));
-  const int pieces = pieces_of(a, r.last_tile - r.first_tile, steps_of_a_piece(a));
+  const int pieces = pieces_of(a, r.last_tile - r.first_tile, steps_of_a_piece<NC>(a));
   if (pieces == 1) return;  // written by the first kernel
   constexpr int kLanes = D / 4, kAtOnce = 64 / kLanes;
   const int lane = threadIdx.x & 63, part = lane / kLanes, d = 4 * (lane % kLanes);
@@ -730,33 +751,36 @@ __global__ void __launch_bounds__(256, 2) attend_prompt_kernel(AttendArgs a) {
 // How a call is laid over the chip, from its sizes alone.
 struct Plan {
   bool prompt;
-  int nc, tiles, waves, splits, least, units;
+  int nc, tiles, waves, search, splits, least;
+  long long units;
   float per_piece;
 };
 Plan plan(int tokens, int seqs, int heads, int kv_heads, int max_query_len, int max_seq_len, int window, int head_size) {
   const long long group = heads / kv_heads, cols = max_query_len * group;
   Plan p;
   p.waves = 4;
+  p.search = 0;
   p.splits = 1;
   p.least = 1;
   p.per_piece = 1.f;
   p.units = seqs;
   // Column tiles of nc x 16, and those of them that hold queries: of all rows together (a batch may mix one prompt with
   // many single tokens), a tile a sequence more where they do not fill their last.
-  long long most_tiles, full, groups;
+  long long most_tiles, full, tiles, groups;
   const auto tile = [&](int nc) {
     p.nc = nc;
     p.tiles = (int)((cols + 16 * nc - 1) / (16 * nc));
     most_tiles = (long long)seqs * p.tiles;
     full = max_query_len == 1 ? most_tiles : (tokens * group + 16 * nc - 1) / (16 * nc);
-    groups = (full + seqs < most_tiles ? full + seqs : most_tiles) * kv_heads;
+    tiles = full + seqs < most_tiles ? full + seqs : most_tiles;
+    groups = tiles * kv_heads;
   };
   tile(cols > 16 ? 2 : 1);
   // A wave for each column tile where these alone fill the chip, two waves a SIMD, and the rows are spread about evenly:
   // 2 x 8 kv heads x 1024 queries of 8 heads take 70 us so and 98 with waves that share the keys, 64 x 8 x 32 queries of
   // 4 heads over 1024 keys 60 and 71.  Below that some SIMDs idle while others have all the keys to run over: one
-  // sequence's 512 queries of 8 x 4 heads over 8192 keys 268 and 102, one query of 128 heads over 65536 keys 2070 and 29;
-  // 2048 queries beside 63 single ones, each over 4096 keys, 995 and 705.  Long sequences want a second such round
+  // sequence's 512 queries of 8 x 4 heads over 8192 keys 268 and 102, one query of 128 heads over 65536 keys 2070 and 27;
+  // 2048 queries beside 63 single ones, each over 4096 keys, 995 and 222.  Long sequences want a second such round
   // (2048 queries of 8 x 4 heads over 65536 keys, one round: 2970 and 2710; twice 2048 over 8192, two: 633 and 630).
   p.prompt = cols > 64 && full * kv_heads >= (max_seq_len > 2048 ? 4096 : 2048) && 2 * full >= most_tiles;
   if (p.prompt) return p;
@@ -778,9 +802,14 @@ Plan plan(int tokens, int seqs, int heads, int kv_heads, int max_query_len, int 
   if (groups * rounds <= 256) p.waves = 8;
   const long long fill = p.nc == 2 ? 512 : head_size == 64 ? 1024 : 768;
   // More short sequences than fill the chip once take fewer waves each, so that it holds more of them: 1024 x 250 keys of
-  // 128 10.4 us with two waves, 13.7 with four, 11.7 with one; 2048 x 129 16.9, 21.5 and 12.6, x 500 30.2, 31.3 and 25.0.
-  if (keys <= 512 && p.nc == 1 && groups > fill) p.waves = groups > 2 * fill ? 1 : 2;
-  if (keys <= (p.waves == 8 ? 2048 : 512)) return p;
+  // 128 10.4 us with two waves, 13.7 with four, 11.7 with one; 2048 x 129 16.9, 21.5 and 12.6, x 500 30.2, 31.3 and 25.0;
+  // 4 x 500 queries of 8 x 4 heads 29.9, 41.4 and 27.4.
+  if (keys <= (p.nc == 2 ? 1024 : 512) && groups > fill) p.waves = groups > 2 * fill ? 1 : 2;
+  // Rows that are spread unevenly would leave workgroups without work, which are looked past: 512 queries beside 63 single
+  // ones, each over 4096 keys, 115 us and 252.
+  p.search = tiles < most_tiles;
+  p.units = p.search ? tiles : seqs;
+  if (keys <= (p.waves == 8 ? 2048 : p.waves == 4 ? 512 : 1024)) return p;
   const long long least = 512, most = (keys + least - 1) / least;
   long long cut = (p.waves == 8 ? 256 : fill) / groups;
   cut = cut < 1 ? 1 : cut;
@@ -791,13 +820,15 @@ Plan plan(int tokens, int seqs, int heads, int kv_heads, int max_query_len, int 
   // 256 x 2048 111 and 90, 127 x 800 35 and 25.  (What is not taken up of a workspace costs nothing; it stays below 2^18
   // pieces of a query head.)
   const long long room = (1LL << 18) / ((long long)tokens * heads);
-  long long splits = cut == 1 && (groups > 1024 || keys <= 2048) ? 1 : most < room ? most : room;
+  long long splits = cut == 1 && (groups > 1024 || keys <= 2048 || seqs == 1) ? 1 : most < room ? most : room;
   p.splits = (int)(splits < 1 ? 1 : splits > 64 ? 64 : splits);
   p.least = (int)(least / kTile);
-  // (half a piece a sequence for the rounding of their numbers: one workgroup too many is a round too many)
-  p.per_piece = 1.f / ((float)kTile * (float)seqs * (cut == 1 ? 1.f : (float)cut - 0.5f));
-  // At most one piece a sequence more than its share, and 2 / 16 for the two tiles that are added to it.
-  p.units = p.splits > 1 ? (int)(seqs * (cut + 1) + (seqs + 3) / 4) : seqs;
+  if (p.splits == 1) return p;
+  // (half a piece a tile for the rounding of their numbers: one workgroup too many is a round too many)
+  p.per_piece = 1.f / ((float)kTile * (float)tiles * (cut == 1 ? 1.f : (float)cut - 0.5f));
+  // At most one piece a tile more than its share, and 2 / 16 for the two steps that are added to it.
+  p.search = 1;
+  p.units = tiles * (cut + 1) + (tiles + 3) / 4;
   return p;
 }
 
@@ -811,7 +842,7 @@ int launch(const AttendArgs& a, const Plan& p, hipStream_t s) {
     hipLaunchKernelGGL((attend_prompt_kernel<T, D, 2>), grid, dim3(256), 0, s, a);
     return serving_after_launch();
   }
-  const dim3 grid((unsigned)p.units * (unsigned)a.kv_heads, (unsigned)p.tiles);
+  const dim3 grid((unsigned)(p.units * a.kv_heads), p.search ? 1u : (unsigned)p.tiles);
   if (p.nc == 1 && p.waves == 1)
     hipLaunchKernelGGL((attend_split_kernel<T, D, 1, 1>), grid, dim3(64), 0, s, a);
   else if (p.nc == 1 && p.waves == 2)
@@ -820,6 +851,10 @@ int launch(const AttendArgs& a, const Plan& p, hipStream_t s) {
     hipLaunchKernelGGL((attend_split_kernel<T, D, 1, 4>), grid, dim3(256), 0, s, a);
   else if (p.nc == 1)
     hipLaunchKernelGGL((attend_split_kernel<T, D, 1, 8>), grid, dim3(512), 0, s, a);
+  else if (p.waves == 1)
+    hipLaunchKernelGGL((attend_split_kernel<T, D, 2, 1>), grid, dim3(64), 0, s, a);
+  else if (p.waves == 2)
+    hipLaunchKernelGGL((attend_split_kernel<T, D, 2, 2>), grid, dim3(128), 0, s, a);
   else if (p.waves == 4)
     hipLaunchKernelGGL((attend_split_kernel<T, D, 2, 4>), grid, dim3(256), 0, s, a);
   else
@@ -869,7 +904,7 @@ extern "C" int serving_attend_kv4(const void* query, long long q_token, long lon
   if (!aligned16(query) || !aligned16(cache) || !aligned16(out) || q_token % 8 || q_head % 8) return SERVING_E_ALIGN;
   const Plan p = plan(tokens, seqs, heads, kv_heads, max_query_len, max_seq_len, window, head_size);
   if ((long long)seqs * kv_heads > 0x7fffffLL || (p.prompt && seqs > 65535) || p.tiles > (p.prompt ? 4 : 1) * 65535LL ||
-      (long long)tokens * heads > 0x7fffffffLL)
+      (!p.prompt && p.units * kv_heads * p.waves * 64 > 0xffffffffLL) || (long long)tokens * heads > 0x7fffffffLL)
     return SERVING_E_TOO_LARGE;
   const size_t need = workspace_of(p, tokens, heads, head_size);
   if (need && (!workspace || workspace_bytes < need)) return SERVING_E_WORKSPACE;
@@ -879,7 +914,7 @@ extern "C" int serving_attend_kv4(const void* query, long long q_token, long lon
                static_cast<float*>(workspace), nullptr, table_width, tokens, seqs, heads, kv_heads, heads / kv_heads,
                (int)num_blocks, block_size,
                sixteens == 1 ? 0u : (uint32_t)(((1ULL << 32) + sixteens - 1) / sixteens),
-               scale * 1.44269504088896340736f, window, max_query_len, p.splits, p.least, p.per_piece};
+               scale * 1.44269504088896340736f, window, max_query_len, p.search, p.splits, p.least, p.per_piece};
   if (need) a.part_ml = a.part_o + (size_t)tokens * heads * p.splits * head_size;
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (head_size == 64) return bf16_in ? launch<bf16, 64>(a, p, s) : launch<f16, 64>(a, p, s);
