@@ -286,3 +286,27 @@ def test_many_short_sequences(ops, cuda, seqs, kv, d, window, dtype):
     case = attend_case(lens, [1] * seqs, kv, kv, d, 16, TYPES[dtype], seqs)
     check_attend(ops, cuda, case, window=window, ragged=False)
     check_attend(ops, cuda, case, window=window, ragged=False, max_seq_len=1)  # (the rest of them is read all the same)
+
+
+@pytest.mark.parametrize("heads,kv,longest,window", [(8, 2, 300, 0), (8, 2, 300, 50), (4, 4, 300, 0), (8, 1, 2600, 0), (8, 1, 2600, 1500)])
+def test_prompts_among_more_sequences_than_lanes(ops, cuda, heads, kv, longest, window):
+    """Prompts before, at and behind the 64th sequence, sequences without rows, rows past the promise."""
+    seqs = 140
+    counts, lens = [1] * seqs, [(13 * i) % 60 + 1 for i in range(seqs)]
+    for at, rows in ((0, 70), (63, 41), (64, 90), (139, 33)):
+        counts[at], lens[at] = rows, longest
+    for at in (7, 62, 65, 128):
+        counts[at] = 0
+    query, cache, tables, lens, start = attend_case(lens, counts, heads, kv, 64, 16, torch.float16, longest)
+    check_attend(ops, cuda, (query, cache, tables, lens, start), window=window)
+    out = torch.full(query.shape, 7.0, dtype=query.dtype, device=cuda)
+    ops.paged_attention_kv4(query.to(cuda), cache.to(cuda), tables.to(cuda), lens.to(cuda), 0.125, longest,
+                            query_start=start.to(cuda), max_query_len=50, window=window, out=out)
+    want, tol = orc.attend(query, cache, tables, lens, start, 0.125, window, True)
+    late = torch.zeros(len(query), dtype=torch.bool)
+    for at in (0, 64):
+        late[int(start[at]) + 50:int(start[at + 1])] = True
+    got = out.cpu().double()
+    assert torch.isnan(got[late]).all()
+    off = int((~((got - want).abs() <= tol))[~late].sum())
+    assert off == 0, off
