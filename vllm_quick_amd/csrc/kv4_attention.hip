@@ -565,6 +565,9 @@ __global__ void __launch_bounds__(64 * WAVES, NC == 1 ? 3 : 2) attend_split_kern
   int b = unit, tile = gridDim.y - 1 - blockIdx.y, split = 0, steps = 1;  // (tiles that see most come first)
   // Without a window the keys begin where they do whatever the length, which is under way meanwhile: one round trip to
   // memory less before the first keys.
+  // Workgroups go to the CUs in turn: sequences in the same order in each row of tiles would give the long ones to the same
+  // CUs again and again (2 x 1024 queries of 8 x 4 heads over 2500 and 8192 keys 269 us, 344 so).
+  if (!a.search && gridDim.y > 2) b = (int)((unsigned)(unit + ((tile * 40503u) >> 5)) % (unsigned)a.seqs);
   const bool ahead = a.window == 0 && !a.search;  // (few tiles are without queries then)
   if (__builtin_expect(a.search, 0)) {
     if (a.splits > 1) steps = steps_of_a_piece<NC>(a);
