@@ -310,3 +310,14 @@ def test_prompts_among_more_sequences_than_lanes(ops, cuda, heads, kv, longest, 
     assert torch.isnan(got[late]).all()
     off = int((~((got - want).abs() <= tol))[~late].sum())
     assert off == 0, off
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("seqs,rows,heads,kv,window", [(90, 7, 32, 8, 0), (90, 7, 32, 8, 20), (40, 20, 32, 8, 0), (70, 9, 24, 8, 0), (33, 5, 160, 16, 0)])
+def test_many_short_sequences_of_several_rows(ops, cuda, seqs, rows, heads, kv, window, dtype):
+    """One and two waves for tiles of 32 columns; evenly spread rows and uneven ones."""
+    counts = [max(1, rows - i % 3) for i in range(seqs)]
+    lens = [c + (7 * i) % 50 for i, c in enumerate(counts)]
+    check_attend(ops, cuda, attend_case(lens, counts, heads, kv, 64, 16, TYPES[dtype], seqs), window=window)
+    counts[1], lens[1] = 3 * rows, 4 * rows
+    check_attend(ops, cuda, attend_case(lens, counts, heads, kv, 64, 16, TYPES[dtype], seqs), window=window)
