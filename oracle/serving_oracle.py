@@ -73,8 +73,9 @@ def store(cache, head_size, slots, key, value):
                 halves[block, h, word], halves[block, h, word + 1] = scale[t, h], least[t, h]
 
 
-def values(cache, head_size, slots):
-    """What slots stand for, in 64 bits: key, value [n, H, D], and the values' scales [n, H] (zeros outside the cache)."""
+def values(cache, head_size, slots, code=None):
+    """What slots stand for, in 64 bits: key, value [n, H, D], and the values' scales [n, H] (zeros outside the cache);
+    what they would with `code` in every element, if given."""
     blocks, heads, size = cache.shape
     p = size // (head_size + 8)
     inside = (slots >= 0) & (slots < blocks * p)
@@ -88,11 +89,12 @@ def values(cache, head_size, slots):
     found, scales = [], []
     for which, byte in enumerate((k_byte, v_byte)):
         raw = cache[block[:, None, None], h[None, :, None], byte[:, None, :]].long()
-        code = (raw >> (4 * (el % 2))) & 15
+        stored = (raw >> (4 * (el % 2))) & 15
         word = (p * head_size + which * 4 * p) // 2 + 2 * at
         scale = halves[block[:, None], h[None], word[:, None]].double()
         least = halves[block[:, None], h[None], word[:, None] + 1].double()
-        x = least[..., None] + code.double() * scale[..., None]
+        x = least[..., None] + (stored.double() if code is None else code) * scale[..., None]
+        x = x.expand(stored.shape)
         found.append(torch.where(inside[:, None, None], x, torch.zeros_like(x)))
         scales.append(scale)
     return found[0], found[1], scales[1]
@@ -149,6 +151,57 @@ def attend(query, cache, tables, lens, start, scale, window, repaired):
                 tol[r0:r0 + m, h] = err + eps * (o.abs() + err) + 2.0**-25
             else:
                 tol[r0:r0 + m, h] = 0
+    return out, tol
+
+
+def attend_counted(query, cache, tables, lens, start, scale, window):
+    """64-bit attention and how far a kernel may be from it, counted key by key, so that keys of very different values
+    may stand beside each other.  The kernel
+      has e_j (the exponential of score j) off by 2 (d + 8) roundings of fp32 of a score's parts, and by 2^-18 for the
+      exponential and for the sum of a score and what it is held against: sum_j p_j |v_j - o| of that,
+      holds w_j = e_j vscale_j in fp16, in a unit that has the largest w_j of the row at 2^6 or more: half a step, 2^-11 of
+      w_j, or 2^-25 of the unit below fp16's normal numbers, times its code; for fp16 results times the code's distance from one that
+      stands between the least value and 0, with which the rounded weight is taken off again.  A product with a code may
+      lose 2^-21 of it,
+      takes sums in fp32: of 64 matrix instructions, of what is set aside every 1024 keys, of 40 waves and pieces, each
+      off by a step of 2^-23 of the sum of absolute values,
+      and rounds the result once.
+    (Rows of no sequence are NaN in both.)"""
+    t, heads, d = query.shape
+    p = cache.shape[2] // (d + 8)
+    group = heads // cache.shape[1]
+    half = query.dtype == torch.float16
+    eps, least_step = torch.finfo(query.dtype).eps / 2, 2.0**-25 if half else 2.0**-60
+    out = torch.full((t, heads, d), float("nan"), dtype=torch.float64)
+    tol = out.clone()
+    for b in range(len(lens)):
+        n, r0 = min(int(lens[b]), tables.shape[1] * p), int(start[b])
+        m = int(start[b + 1]) - r0
+        j = torch.arange(max(n, 0))
+        slots = tables[b].long()[j // p] * p + j % p
+        keys, values_, scales = values(cache, d, slots)
+        leasts = values(cache, d, slots, 0.0)[1]
+        for r in range(m):
+            last = n - m + r
+            see = j[max(0, last + 1 - window if window else 0):max(0, last + 1)]
+            if not len(see):
+                out[r0 + r] = tol[r0 + r] = 0
+                continue
+            for h in range(heads):
+                q = query[r0 + r, h].double()
+                k, v, vs, least = (x[see, h // group] for x in (keys, values_, scales, leasts))
+                pr = torch.softmax((k @ q) * scale, 0)
+                o = pr @ v
+                size = abs(scale) * q.abs().sum() * k.abs().max()
+                moved = 2 * (2 * (d + 8) * 2.0**-24 * 3 * size + 2.0**-18)
+                codes = pr @ (v - least)
+                apart = pr @ torch.minimum(v.abs() + least.abs(), 15 * vs[:, None]) if half else codes
+                sums = codes + 3 * (pr @ least.abs())
+                err = moved * (pr @ (v - o).abs()) + 2.0**-11 * apart + 2.0**-21 * codes
+                err += 15 * len(see) * (2.0**-31 * (pr * vs).max() + 2.0**-55)
+                err += (104 + len(see) / 1024) * 2.0**-23 * (sums + o.abs())
+                out[r0 + r, h] = o
+                tol[r0 + r, h] = err + eps * (o.abs() + err) + least_step
     return out, tol
 
 

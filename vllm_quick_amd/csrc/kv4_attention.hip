@@ -20,10 +20,12 @@
 //                  piece, so that the same 4 keys of a piece are again one 16-byte load, and one byte permutation a
 //                  word pairs the codes of neighbouring keys.
 // Roundings: queries enter exactly (scaled by a power of two into fp16's range), w_j = p_j vscale_j is rounded to fp16
-// once, all sums are fp32.  For fp16 results the other two sums, of p_j and of p_j vleast_j, take what w_j became divided
-// by vscale_j (to an eighth of the difference) in place of p_j: a rounding then weighs a key by a little more or less, by
-// all elements and the denominator alike, where otherwise it would cost up to 15 steps of the codes.  bf16 results are
-// rounded coarser than that.
+// once, all sums are fp32.  What a rounding takes from w_j or adds to it, its code multiplies, by up to 15.  For fp16 results
+//   o = sum_j w_j (code_j - zero_j) + sum_j p_j (vleast_j + zero_j vscale_j),
+// with zero_j near the code that would stand for 0 (any number is right), and w_j zero_j taken off with the rounded w_j, in a
+// matrix instruction of its own: a rounding then costs about its share of the value, and nothing that the sum of p_j or the
+// second sum take depends on it, however small w_j is.  bf16 results are rounded coarser than that.  2 x 2048 queries of 64
+// heads of 128 take 760 us so in fp16, 720 with 7.5 for every zero_j (and 1.4 times the error), 700 without.
 #include "kv4_cache.h"
 
 namespace {
@@ -63,9 +65,12 @@ typedef const __attribute__((address_space(4))) int32_t* scalar_ints;
 __device__ __forceinline__ scalar_ints scalar(const int32_t* p) { return (scalar_ints)(uintptr_t)p; }
 __device__ __forceinline__ f16x2 as_pair(uint32_t w) { return __builtin_bit_cast(f16x2, w); }  // scale, least
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
-// 1 / v to an eighth of it, from the number's bits: the line of slope -1 through (log2 v, log2 1/v) that is nearest.
-__device__ __forceinline__ float rough_reciprocal(float v) {
-  return __builtin_bit_cast(float, 0x7ef311c7u - __builtin_bit_cast(uint32_t, v));
+// least / scale of two keys within -15 .. 0, to an eighth of it where the scale is a normal number: 1 / scale from the
+// number's bits, the line of slope -1 through (log2 v, log2 1/v) that is nearest.
+__device__ __forceinline__ f16x2 minus_zero(uint32_t scales, f16x2 leasts) {
+  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+  const f16x2 z = leasts * __builtin_bit_cast(f16x2, u16x2{0x7798, 0x7798} - __builtin_bit_cast(u16x2, scales));
+  return __builtin_elementwise_min(__builtin_elementwise_max(z, f16x2{(f16)-15.f, (f16)-15.f}), f16x2{(f16)0.f, (f16)0.f});
 }
 __device__ __forceinline__ float over_groups_max(float v) {  // of the four groups of 16 lanes
   v = fmaxf(v, __shfl_xor(v, 16));
@@ -102,7 +107,7 @@ template <typename T, int D, int NC, bool ONCE>
 struct Wave {
   static constexpr int kSteps = D / 32;  // matrix instructions of 16 keys against 16 columns
   static constexpr int kRows = D / 16;   // tiles of 16 elements of the result
-  static constexpr bool kRepair = __is_same(T, f16);
+  static constexpr bool kCentred = __is_same(T, f16);
 
   const AttendArgs& a;
   const int c, g;
@@ -119,7 +124,7 @@ struct Wave {
   float* kept;                        // in LDS: [16 NC][D + 4], what was set aside of the sums of p v,
   float kept_sum[NC], kept_shift[NC];  // of p, and the shift that both go with
   bool keeps;
-  f32x4 o[NC][kRows];
+  f32x4 o[NC][kRows], off[NC];  // sums of w code and, in each element, of w (- zero) (kCentred)
   float vref;                // power of two above every vscale so far,
   float weight_log;          // and what p's are held at for it: p vscale 2^weight_log is below 2^(kSlack + kWeightLog)
   const uint8_t* head_base;  // of this kv head in block 0
@@ -200,6 +205,7 @@ struct Wave {
       sum[n] = flat[n] = 0.f;
 #pragma unroll
       for (int m = 0; m < kRows; ++m) o[n][m] = f32x4{0.f, 0.f, 0.f, 0.f};
+      off[n] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
   }
 
@@ -267,9 +273,11 @@ struct Wave {
     return key >= low[n] && key < lim[n];
   }
 
-  // Scores of 32 keys to weights, the B operand of the second product.  ks: the keys' scales in the unit of the scores.
+  // Scores of 32 keys to weights, the B operand of the second product.  ks: the keys' scales in the unit of the scores;
+  // level: what the values' codes of zero stand for (kCentred).
   template <bool MASK>
-  __device__ __forceinline__ void weigh(const f32x4 (&s)[2], int n, int from, const float (&ks)[8], f16x8& p) {
+  __device__ __forceinline__ void weigh(const f32x4 (&s)[2], int n, int from, const float (&ks)[8], const float (&level)[8],
+                                        f16x8& p) {
     float t[8];
     const auto score = [&](int i, float more) {
       return __builtin_fmaf(ks[i], s[i / 4][i % 4], __builtin_fmaf((float)as_pair(kp[i / 4][i % 4]).y, qs[n], more));
@@ -295,6 +303,7 @@ struct Wave {
       flat[n] *= f;
 #pragma unroll
       for (int m = 0; m < kRows; ++m) o[n][m] *= f;
+      off[n] *= f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {  // (rounded as outside of this branch, which other columns may have called for)
         t[i] = score(i, next);
@@ -304,7 +313,7 @@ struct Wave {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const f16x2 par = as_pair(vp[i / 4][i % 4]);
-      float e = exp2_(t[i]), w = e * (float)par.x, least = (float)par.y;
+      float e = exp2_(t[i]), w = e * (float)par.x, least = kCentred ? level[i] : (float)par.y;
       if (MASK) {  // (not 0 times what a hidden key's parameters may be)
         const bool on = sees(n, from, i);
         e = on ? e : 0.f;
@@ -312,7 +321,6 @@ struct Wave {
         least = on ? least : 0.f;
       }
       p[i] = (f16)w;
-      if (kRepair) e = __builtin_fmaf((float)p[i] - w, rough_reciprocal(fmaxf((float)par.x, 0x1p-40f)), e);
       sum[n] += e;
       flat[n] = __builtin_fmaf(e, least, flat[n]);
     }
@@ -360,6 +368,7 @@ struct Wave {
         flat[n] *= f;
 #pragma unroll
         for (int m = 0; m < kRows; ++m) o[n][m] *= f;
+        off[n] *= f;
       }
     }
     float ks[8];
@@ -368,9 +377,20 @@ struct Wave {
       ks[i] = (float)as_pair(kp[i / 4][i % 4]).x * unit_score;
       if (MASK && !known_now[i / 4]) ks[i] = __builtin_nanf("");  // of a block that the cache does not have
     }
-    f16x8 p[NC];
+    f16x8 p[NC], zero;  // (zero: negative)
+    float level[8];
+    if (kCentred) {
 #pragma unroll
-    for (int n = 0; n < NC; ++n) weigh<MASK>(s[n], n, from, ks, p[n]);
+      for (int i = 0; i < 8; i += 2) {
+        const uint32_t a0 = vp[i / 4][i % 4], a1 = vp[i / 4][i % 4 + 1];
+        const f16x2 z = minus_zero(__builtin_amdgcn_perm(a1, a0, 0x05040100u), as_pair(__builtin_amdgcn_perm(a1, a0, 0x07060302u)));
+        zero[i] = z.x, zero[i + 1] = z.y;
+        level[i] = __builtin_fmaf((float)as_pair(a0).x, -(float)z.x, (float)as_pair(a0).y);
+        level[i + 1] = __builtin_fmaf((float)as_pair(a1).x, -(float)z.y, (float)as_pair(a1).y);
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < NC; ++n) weigh<MASK>(s[n], n, from, ks, level, p[n]);
     load_params();
     // pairs of neighbouring keys side by side: 16 bits (4 elements) of each in one word
 #pragma unroll
@@ -389,6 +409,11 @@ struct Wave {
       }
     }
     load_values();
+    if (kCentred) {
+#pragma unroll
+      for (int n = 0; n < NC; ++n)
+        off[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(zero, p[n], off[n], 0, 0, 0);
+    }
   }
 
   // Runs over tiles first, first + stride, .. < last, the first of them loaded; all columns see all of the tiles that lie
@@ -445,6 +470,7 @@ struct Wave {
       sum[n] = flat[n] = 0.f;
 #pragma unroll
       for (int m = 0; m < kRows; ++m) o[n][m] = f32x4{0.f, 0.f, 0.f, 0.f};
+      off[n] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
     keeps = true;
   }
@@ -453,7 +479,7 @@ struct Wave {
   template <typename F>
   __device__ __forceinline__ void results(int n, F&& out) {
     constexpr int kEach = kRows;  // neighbouring elements that a lane holds: element kEach (4 g + r) + m
-    const float rest = over_groups_sum(flat[n]);
+    const float rest = kCentred ? over_groups_sum(flat[n]) + off[n][0] : over_groups_sum(flat[n]);
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       float x[kEach];
@@ -555,7 +581,7 @@ __device__ void refuse_rows(const AttendArgs& a, const Sequence& s, int kv) {
 // 64 sequences of up to 4096 keys, 32 kv heads of 128, takes 114 us (5.1 TB/s; a kernel that only reads reaches 5.7), of 8
 // sequences of up to 65536, 8 kv heads, 68 us (6.0) and 6 of the join.
 template <typename T, int D, int NC, int WAVES>
-__global__ void __launch_bounds__(64 * WAVES, NC == 1 ? 3 : 2) attend_split_kernel(AttendArgs a) {
+__global__ void __launch_bounds__(64 * WAVES, NC == 1 || D == 64 ? 3 : 2) attend_split_kernel(AttendArgs a) {
   constexpr int kCols = 16 * NC;
   __shared__ float part[WAVES][kCols][D + 4];
   __shared__ float maxima[WAVES][kCols], sums[WAVES][kCols];
@@ -710,7 +736,7 @@ __device__ __forceinline__ int by_length(const AttendArgs& a, int rank) {
 // 8192 keys take 708 us, 0.78 PFLOP/s.  Converting each code once a workgroup, through LDS, takes a quarter of them away
 // and costs more in waits than that (740 us with two barriers a step).
 template <typename T, int D, int NC>
-__global__ void __launch_bounds__(256, 2) attend_prompt_kernel(AttendArgs a) {
+__global__ void __launch_bounds__(256, D == 64 ? 3 : 2) attend_prompt_kernel(AttendArgs a) {
   constexpr int kCols = 16 * NC;
   __shared__ float part[4][kCols][D + 4];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
