@@ -72,10 +72,10 @@ def case_of(form, dtype, large, small, share, where):
     return in_a_large_batch(case, 2048) if many else case
 
 
-def run(ops, cuda, case, rows, scale):
+def run(ops, cuda, case, rows, scale, window=0):
     query, cache, tables, lens, start = case
     return ops.paged_attention_kv4(query.to(cuda), cache.to(cuda), tables.to(cuda), lens.to(cuda), scale, int(lens.max()),
-                                   query_start=start.to(cuda) if rows > 1 else None, max_query_len=rows).cpu()
+                                   query_start=start.to(cuda) if rows > 1 else None, max_query_len=rows, window=window).cpu()
 
 
 def some_of(case):
@@ -91,11 +91,11 @@ def some_of(case):
     return parts
 
 
-def check(ops, cuda, form, case, scale=None):
+def check(ops, cuda, form, case, scale=None, window=0):
     scale = FORMS[form][4]**-0.5 if scale is None else scale
-    got = run(ops, cuda, case, FORMS[form][1], scale).double()
+    got = run(ops, cuda, case, FORMS[form][1], scale, window).double()
     for at, part in some_of(case):
-        want, tol = orc.attend_counted(*part, scale, 0)
+        want, tol = orc.attend_counted(*part, scale, window)
         off = (got[at] - want).abs() / tol
         assert not (off > 1).any() and not torch.isnan(off).any(), f"{float((off > 1).double().mean()):.3f} of the results off, worst {float(off.max()):.3g} of what is allowed"
 
@@ -110,8 +110,6 @@ def check(ops, cuda, form, case, scale=None):
 ])
 @pytest.mark.parametrize("form", FORMS)
 def test_a_large_token_that_is_attended_to(ops, cuda, form, large, small, share, where):
-    if where == "last" and FORMS[form][1] > 1:
-        pytest.skip("other rows do not see the last token")
     for dtype in TYPES.values():
         check(ops, cuda, form, case_of(form, dtype, large, small, share, where))
 
@@ -125,3 +123,55 @@ def test_a_large_token_among_many(ops, cuda):
                 check(ops, cuda, "many", case_of("many", dtype, large, small, share, "first"))
     finally:
         del FORMS["many"]
+
+
+@pytest.mark.parametrize("where", ["first", "between", "last"])
+@pytest.mark.parametrize("large,small,share", [
+    (6000.0, 1e-4, -24),
+    (15000.0, 1e-3, -30),
+    (15000.0, 1e-6, -45),
+    (100.0, 1e-4, -13),
+])
+@pytest.mark.parametrize("form", FORMS)
+def test_a_large_token_that_is_hardly_attended_to(ops, cuda, form, large, small, share, where):
+    for dtype in TYPES.values():
+        check(ops, cuda, form, case_of(form, dtype, large, small, share, where))
+
+
+@pytest.mark.parametrize("large,small,share", [(15000.0, 1e-3, 0), (6000.0, 1e-4, 6)])
+@pytest.mark.parametrize("form", [f for f in FORMS if FORMS[f][1] > 1])
+def test_a_large_token_that_a_window_leaves_behind(ops, cuda, form, large, small, share):
+    """The first rows of a sequence see it, the last ones do not."""
+    _, rows, _, _, _, n, _ = FORMS[form]
+    for dtype in TYPES.values():
+        check(ops, cuda, form, case_of(form, dtype, large, small, share, "first"), window=n - rows // 2 - 4)
+
+
+@pytest.mark.parametrize("size", [1.0, 2.0**-10])
+@pytest.mark.parametrize("form", [f for f in FORMS if FORMS[f][1] > 1])
+def test_what_rows_do_not_see_changes_no_bit_of_them(ops, cuda, form, size):
+    """Heads of the largest scale that fp16 holds, or of NaN, in the last token of each sequence, which its last row alone
+    sees, or in the first one, which a window hides from it."""
+    _, rows, _, kv, d, n, _ = FORMS[form]
+    wide = torch.full((1, kv, d), 6e4)
+    wide[..., ::2] = -6e4
+    for dtype in TYPES.values():
+        case = case_of(form, dtype, size, size, 0, "first")
+        query, cache, tables, lens, start = case
+        last = start[1:].long() - 1
+        others = torch.ones(int(start[-1]), dtype=torch.bool)
+        others[last] = False
+        for at, window, kept in (("last", 0, others), ("first", n - 4, ~others)):
+            # (lengths differ: the shortest sequences' last rows see their first token through this window)
+            kept = kept.clone()
+            if at == "first":
+                kept[last[lens <= n - 4]] = False
+            base = run(ops, cuda, case, rows, d**-0.5, window)[:int(start[-1])]
+            for x in (wide, torch.full((1, kv, d), float("nan"))):
+                other = cache.clone()
+                for b, length in enumerate(lens.tolist()):
+                    j = length - 1 if at == "last" else 0
+                    orc.store(other, d, tables[b, j // 16].long().view(1) * 16 + j % 16, x, x)
+                got = run(ops, cuda, (query, other, tables, lens, start), rows, d**-0.5, window)[:int(start[-1])]
+                assert torch.equal(got[kept], base[kept]) and not torch.isnan(base).any()
+                assert not torch.equal(got[~kept], base[~kept])

@@ -25,7 +25,7 @@
 // with zero_j near the code that would stand for 0 (any number is right), and w_j zero_j taken off with the rounded w_j, in a
 // matrix instruction of its own: a rounding then costs about its share of the value, and nothing that the sum of p_j or the
 // second sum take depends on it, however small w_j is.  bf16 results are rounded coarser than that.  2 x 2048 queries of 64
-// heads of 128 take 760 us so in fp16, 720 with 7.5 for every zero_j (and 1.4 times the error), 700 without.
+// heads of 128 take 755 us so in fp16, some 40 less with 7.5 for every zero_j (and 1.4 times the error), 700 in bf16.
 #include "kv4_cache.h"
 
 namespace {
@@ -35,8 +35,9 @@ using namespace serving;
 constexpr float kNone = -1e30f;  // below every score, yet finite: differences of it are numbers
 constexpr int kTile = 32;        // keys of a step
 constexpr int kRun = 32;         // steps between two settings aside
-constexpr float kSlack = 8.f;     // a probability may stand this many powers of two above 1 before the maximum moves
-constexpr float kWeightLog = 7.f;  // p vscale / (power of two above vscale) 2^7 is rounded to fp16: below 2^15
+constexpr float kWeightLog = 7.f;      // what a column is held against is set so that no p vscale of a step passes 2^7,
+constexpr float kMostWeight = 15.f;    // and again when one may pass 2^15, which fp16 holds
+constexpr float kLeastScale = 0x1p-24f;  // of a token whose values are all alike, for that purpose: fp16's least number
 
 struct AttendArgs {
   const void* query;
@@ -118,15 +119,13 @@ struct Wave {
   float qs[NC];          // sum of the query, in the unit of the scores
   int lim[NC], low[NC];  // keys that a column sees: low .. lim - 1
   int least_low;         // of all columns of the wave
-  float shift[NC];       // p 2^weight_log = 2^(score + shift): no p passes 2^kSlack
+  float shift[NC];       // p = 2^(score + shift)
   float sum[NC], flat[NC];
   float unit_score;      // what makes a score (in powers of two) of a product
   float* kept;                        // in LDS: [16 NC][D + 4], what was set aside of the sums of p v,
   float kept_sum[NC], kept_shift[NC];  // of p, and the shift that both go with
   bool keeps;
   f32x4 o[NC][kRows], off[NC];  // sums of w code and, in each element, of w (- zero) (kCentred)
-  float vref;                // power of two above every vscale so far,
-  float weight_log;          // and what p's are held at for it: p vscale 2^weight_log is below 2^(kSlack + kWeightLog)
   const uint8_t* head_base;  // of this kv head in block 0
   scalar_ints table;
   long long block_bytes;
@@ -156,8 +155,6 @@ struct Wave {
   __device__ __forceinline__ void begin(const Sequence& s, int kv, int col0, int cols) {
     last_page = max(0, page_of((s.length - 1) >> 4));
     least_low = a.window > 0 ? max(0, s.before + col0 / a.group + 1 - a.window) : 0;
-    vref = 0x1p-40f;
-    weight_log = kWeightLog + 40.f;
     float x[NC][kSteps][8], big = 0.f;
     const float sign = a.scale < 0.f ? -1.f : 1.f;
 #pragma unroll
@@ -274,10 +271,11 @@ struct Wave {
   }
 
   // Scores of 32 keys to weights, the B operand of the second product.  ks: the keys' scales in the unit of the scores;
-  // level: what the values' codes of zero stand for (kCentred).
+  // level: what the values' codes of zero stand for (kCentred); limit: no p above 2^limit makes a p vscale of this lane
+  // pass 2^kMostWeight.
   template <bool MASK>
   __device__ __forceinline__ void weigh(const f32x4 (&s)[2], int n, int from, const float (&ks)[8], const float (&level)[8],
-                                        f16x8& p) {
+                                        float limit, f16x8& p) {
     float t[8];
     const auto score = [&](int i, float more) {
       return __builtin_fmaf(ks[i], s[i / 4][i % 4], __builtin_fmaf((float)as_pair(kp[i / 4][i % 4]).y, qs[n], more));
@@ -290,13 +288,19 @@ struct Wave {
     float most = t[0];
 #pragma unroll
     for (int i = 1; i < 8; ++i) most = fmaxf(most, t[i]);
-    if (__any(most > kSlack + weight_log)) {
+    if (__any(most > limit)) {
       stay();
-      most = kNone;
+      float passed = kNone, top = kNone;  // of score + log2 vscale, or a little above it
 #pragma unroll
-      for (int i = 0; i < 8; ++i) most = !MASK || sees(n, from, i) ? fmaxf(most, score(i, 0.f)) : most;
-      most = over_groups_max(most);  // (a column moves for its own keys only, whatever the wave's others do)
-      const float next = most + shift[n] > kSlack + weight_log ? weight_log - most : shift[n];
+      for (int i = 0; i < 8; ++i) {
+        uint32_t par = vp[i / 4][i % 4];
+        asm volatile("" : "+v"(par));  // (worked out here, not kept in registers for here)
+        const float log_scale = (float)__builtin_amdgcn_frexp_expf(fmaxf((float)as_pair(par).x, kLeastScale));
+        passed = fmaxf(passed, t[i] + log_scale);
+        if (!MASK || sees(n, from, i)) top = fmaxf(top, score(i, log_scale));
+      }
+      // (a column moves for its own keys only, whatever the wave's others do)
+      const float next = over_groups_max(passed) > kMostWeight ? kWeightLog - over_groups_max(top) : shift[n];
       const float f = exp2_(next - shift[n]);
       shift[n] = next;
       sum[n] *= f;
@@ -326,9 +330,10 @@ struct Wave {
     }
   }
 
-  // 32 keys.  What the running maximum and the values' scales are measured against moves only when a probability would
-  // pass 2^kSlack, or a scale its reference, which no step but the first few does: the four groups of lanes need to
-  // agree on neither until then.
+  // 32 keys.  What a column is held against, the running maximum of p vscale over the keys that it sees, moves only when one
+  // would pass 2^8 of it, which no step but the first few does: the four groups of lanes need not agree on it until then.
+  // (The maximum of the product: a key of a large scale that is hardly attended to, or not seen, must not cost the others
+  // their digits in fp16.)
   template <bool MASK>
   __device__ __forceinline__ void step(int from, int length) {
     f32x4 s[NC][2];
@@ -355,22 +360,7 @@ struct Wave {
     f16x2 big = as_pair(vp[0][0]);
 #pragma unroll
     for (int i = 1; i < 8; ++i) big = __builtin_elementwise_max(big, as_pair(vp[i / 4][i % 4]));
-    if (__any((float)big.x >= vref)) {
-      stay();
-      const int to = __builtin_amdgcn_frexp_expf(over_groups_max((float)big.x));  // 2^to is above every scale
-      const float f = vref * __builtin_ldexpf(1.f, -to), log_f = kWeightLog - (float)to - weight_log;
-      vref = __builtin_ldexpf(1.f, to);
-      weight_log = kWeightLog - (float)to;
-#pragma unroll
-      for (int n = 0; n < NC; ++n) {
-        shift[n] = shift[n] >= -kNone ? shift[n] : shift[n] + log_f;
-        sum[n] *= f;
-        flat[n] *= f;
-#pragma unroll
-        for (int m = 0; m < kRows; ++m) o[n][m] *= f;
-        off[n] *= f;
-      }
-    }
+    const float limit = kMostWeight - (float)__builtin_amdgcn_frexp_expf(fmaxf((float)big.x, kLeastScale));
     float ks[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -390,7 +380,7 @@ struct Wave {
       }
     }
 #pragma unroll
-    for (int n = 0; n < NC; ++n) weigh<MASK>(s[n], n, from, ks, level, p[n]);
+    for (int n = 0; n < NC; ++n) weigh<MASK>(s[n], n, from, ks, level, limit, p[n]);
     load_params();
     // pairs of neighbouring keys side by side: 16 bits (4 elements) of each in one word
 #pragma unroll
@@ -475,7 +465,7 @@ struct Wave {
     keeps = true;
   }
 
-  // Element d of the result of this lane's column, as sums of p v 2^weight_log: out(first of kEach elements, values).
+  // Element d of the result of this lane's column, as sums of p v: out(first of kEach elements, values).
   template <typename F>
   __device__ __forceinline__ void results(int n, F&& out) {
     constexpr int kEach = kRows;  // neighbouring elements that a lane holds: element kEach (4 g + r) + m
