@@ -175,3 +175,13 @@ def test_what_rows_do_not_see_changes_no_bit_of_them(ops, cuda, form, size):
                 got = run(ops, cuda, (query, other, tables, lens, start), rows, d**-0.5, window)[:int(start[-1])]
                 assert torch.equal(got[kept], base[kept]) and not torch.isnan(base).any()
                 assert not torch.equal(got[~kept], base[~kept])
+
+
+@pytest.mark.parametrize("size", [1e4, 1e6, 1e8, 1e10, 1e20, 1e31, -1e9, -1e31])
+@pytest.mark.parametrize("form", FORMS)
+def test_scores_of_any_size(ops, cuda, form, size):
+    """Scores so far apart that one token of each row has all the weight (to what 64 bits say); bf16 queries, whose type
+    has the range."""
+    query, *rest = case_of(form, torch.float32, 1.0, 1.0, 0, "first")
+    query = (query * (abs(size) if abs(size) > 1e10 else 1.0)).bfloat16()
+    check(ops, cuda, form, (query, *rest), scale=math.copysign(1.0, size) if abs(size) > 1e10 else size)

@@ -32,12 +32,16 @@ namespace {
 
 using namespace serving;
 
-constexpr float kNone = -1e30f;  // below every score, yet finite: differences of it are numbers
+constexpr float kNone = -0x1p127f;  // below every score, yet finite: differences of it are numbers
 constexpr int kTile = 32;        // keys of a step
 constexpr int kRun = 32;         // steps between two settings aside
 constexpr float kWeightLog = 7.f;      // what a column is held against is set so that no p vscale of a step passes 2^7,
 constexpr float kMostWeight = 15.f;    // and again when one may pass 2^15, which fp16 holds
 constexpr float kLeastScale = 0x1p-24f;  // of a token whose values are all alike, for that purpose: fp16's least number
+
+// Scores beyond kFar have digits of 4 and more: what fp16 holds of a weight would be their roundings'.  A query whose
+// absolute values, times the scale, stay below 2^-17 of it in sum has none (a key is below 2^17).
+constexpr float kFar = 0x1p25f;
 
 struct AttendArgs {
   const void* query;
@@ -125,6 +129,7 @@ struct Wave {
   float* kept;                        // in LDS: [16 NC][D + 4], what was set aside of the sums of p v,
   float kept_sum[NC], kept_shift[NC];  // of p, and the shift that both go with
   bool keeps;
+  bool far;  // some column's scores may pass kFar: all steps are taken as those with masks then, which see to it
   f32x4 o[NC][kRows], off[NC];  // sums of w code and, in each element, of w (- zero) (kCentred)
   const uint8_t* head_base;  // of this kv head in block 0
   scalar_ints table;
@@ -155,7 +160,7 @@ struct Wave {
   __device__ __forceinline__ void begin(const Sequence& s, int kv, int col0, int cols) {
     last_page = max(0, page_of((s.length - 1) >> 4));
     least_low = a.window > 0 ? max(0, s.before + col0 / a.group + 1 - a.window) : 0;
-    float x[NC][kSteps][8], big = 0.f;
+    float x[NC][kSteps][8], big = 0.f, reach = 0.f;
     const float sign = a.scale < 0.f ? -1.f : 1.f;
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
@@ -166,7 +171,7 @@ struct Wave {
       low[n] = a.window > 0 ? max(0, lim[n] - a.window) : 0;
       const T* src = static_cast<const T*>(a.query) + (long long)(s.row + qi) * a.q_token + (kv * a.group + h) * a.q_head;
       typedef T vec8 __attribute__((ext_vector_type(8)));
-      float most = 0.f, total = 0.f;
+      float most = 0.f, total = 0.f, size = 0.f;
 #pragma unroll
       for (int j = 0; j < kSteps; ++j) {
         vec8 w = {};
@@ -175,14 +180,17 @@ struct Wave {
         for (int i = 0; i < 8; ++i) {
           x[n][j][i] = sign * (float)w[i];
           most = fmaxf(most, fabsf(x[n][j][i]));
+          size += fabsf(x[n][j][i]);
           total += x[n][j][i];
         }
       }
       qs[n] = over_groups_sum(total);
+      reach = fmaxf(reach, over_groups_sum(size));
       big = fmaxf(big, most < __builtin_inff() ? most : 0.f);  // (an infinite query is its own column's affair)
     }
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) big = fmaxf(big, __shfl_xor(big, m));
+    far = __any(!(reach * fabsf(a.scale) * 0x1p17f < kFar));
     // All columns by one power of two, the largest element into [2^13, 2^14): a sixteenth of it, and of what is far below
     // it, is still a normal fp16 number, and what is not is 2^-38 of the largest score.
     const int e = 14 - __builtin_amdgcn_frexp_expf(big);
@@ -282,7 +290,7 @@ struct Wave {
     };
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      t[i] = score(i, shift[n]);
+      t[i] = MASK ? score(i, 0.f) + shift[n] : score(i, shift[n]);  // (a far score is rounded alike whatever is added)
       if (MASK) t[i] = sees(n, from, i) ? t[i] : kNone;
     }
     float most = t[0];
@@ -290,17 +298,25 @@ struct Wave {
     for (int i = 1; i < 8; ++i) most = fmaxf(most, t[i]);
     if (__any(most > limit)) {
       stay();
-      float passed = kNone, top = kNone;  // of score + log2 vscale, or a little above it
+      float passed = kNone, top = kNone, peak = kNone;  // of score + log2 vscale, or a little above it; of scores
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         uint32_t par = vp[i / 4][i % 4];
         asm volatile("" : "+v"(par));  // (worked out here, not kept in registers for here)
         const float log_scale = (float)__builtin_amdgcn_frexp_expf(fmaxf((float)as_pair(par).x, kLeastScale));
         passed = fmaxf(passed, t[i] + log_scale);
-        if (!MASK || sees(n, from, i)) top = fmaxf(top, score(i, log_scale));
+        if (MASK && !sees(n, from, i)) continue;
+        const float x = MASK ? score(i, 0.f) : 0.f;
+        peak = fmaxf(peak, x);
+        top = fmaxf(top, MASK ? x + log_scale : score(i, log_scale));
       }
       // (a column moves for its own keys only, whatever the wave's others do)
-      const float next = over_groups_max(passed) > kMostWeight ? kWeightLog - over_groups_max(top) : shift[n];
+      const bool moves = over_groups_max(passed) > kMostWeight;
+      float next = moves ? kWeightLog - over_groups_max(top) : shift[n];
+      if (MASK) {
+        peak = over_groups_max(peak);
+        if (moves && fabsf(peak) >= kFar) next = -peak;
+      }
       const float f = exp2_(next - shift[n]);
       shift[n] = next;
       sum[n] *= f;
@@ -310,7 +326,7 @@ struct Wave {
       off[n] *= f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {  // (rounded as outside of this branch, which other columns may have called for)
-        t[i] = score(i, next);
+        t[i] = MASK ? score(i, 0.f) + next : score(i, next);
         if (MASK) t[i] = sees(n, from, i) ? t[i] : kNone;
       }
     }
@@ -408,6 +424,8 @@ struct Wave {
 
   // Runs over tiles first, first + stride, .. < last, the first of them loaded; all columns see all of the tiles that lie
   // in whole_from .. whole_to - 1 of the keys.
+  // ALONE: a wave runs over all the keys by itself, which makes setting aside worth its place where scores are far too.
+  template <bool ALONE>
   __device__ __forceinline__ void run(int first, int last, int stride, int length, int whole_from, int whole_to) {
     if (first >= last) return;
     int next = min(first + stride, last - 1);  // (the last step loads some tile again, which nobody looks at)
@@ -418,9 +436,9 @@ struct Wave {
       b0 = block_of(2 * next), b1 = block_of(2 * next + 1);
     };
     const int whole_first = (whole_from + kTile - 1) / kTile, whole_last = min(last, whole_to / kTile);
-    int i = first;
+    int i = first, masked = 0;
     while (true) {
-      if (i >= whole_first) {
+      if (i >= whole_first && !far) {
         const int stop = min(whole_last, i + kRun * stride);
         for (; i < stop && known[0] && known[1]; i += stride) {
           advance();
@@ -436,6 +454,7 @@ struct Wave {
       step<true>(i * kTile, length);
       i += stride;
       if (i >= last) break;
+      if (ALONE && far && ++masked % kRun == 0) set_aside();
     }
   }
 
@@ -602,7 +621,7 @@ __global__ void __launch_bounds__(64 * WAVES, NC == 1 || D == 64 ? 3 : 2) attend
   const int t0 = r.first_tile + all * split / pieces + wave, t1 = r.first_tile + all * (split + 1) / pieces;
   if (!ahead) w.first_loads(b, kv, t0, &part[wave][0][0]);
   w.begin(s, kv, col0, cols);
-  w.run(t0, t1, WAVES, s.length, r.whole_from, r.whole_to);
+  w.template run<false>(t0, t1, WAVES, s.length, r.whole_from, r.whole_to);
 
   w.set_aside();
 #pragma unroll
@@ -678,7 +697,7 @@ __global__ void __launch_bounds__(256) attend_join_kernel(AttendArgs a) {
   constexpr int kLanes = D / 4, kAtOnce = 64 / kLanes;
   const int lane = threadIdx.x & 63, part = lane / kLanes, d = 4 * (lane % kLanes);
   const float* ml = a.part_ml + (long long)at * a.splits * 2;
-  float most = -1e38f, total = 0.f;
+  float most = kNone, total = 0.f;
   if (lane < pieces) most = ml[2 * lane], total = ml[2 * lane + 1];
   float top = most;
 #pragma unroll
@@ -743,7 +762,7 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2) attend_prompt_kernel(Att
   Wave<T, D, NC, false> w(a);
   w.first_loads(b, kv, r.first_tile, &part[wave][0][0]);
   w.begin(s, kv, col0, cols);
-  w.run(r.first_tile, r.last_tile, 1, s.length, r.whole_from, r.whole_to);
+  w.template run<true>(r.first_tile, r.last_tile, 1, s.length, r.whole_from, r.whole_to);
   if (w.keeps) w.set_aside();
 #pragma unroll
   for (int n = 0; n < NC; ++n) {
