@@ -185,3 +185,18 @@ def test_scores_of_any_size(ops, cuda, form, size):
     query, *rest = case_of(form, torch.float32, 1.0, 1.0, 0, "first")
     query = (query * (abs(size) if abs(size) > 1e10 else 1.0)).bfloat16()
     check(ops, cuda, form, (query, *rest), scale=math.copysign(1.0, size) if abs(size) > 1e10 else size)
+
+
+@pytest.mark.parametrize("large", [0, 1, -1])
+@pytest.mark.parametrize("form", [f for f in FORMS if FORMS[f][2] * FORMS[f][1] > FORMS[f][3]])
+def test_a_query_that_is_far_larger_than_its_neighbours(ops, cuda, form, large):
+    """One head of one row (of each sequence) 10^9, 10^12 or 10^30 times, in fp16 10^6 times the others, which share its tile."""
+    seqs, rows, heads, _, d, _, _ = FORMS[form]
+    for dtype, low, high in (("bf16", 1.0, 1e9), ("bf16", 1.0, 1e12), ("bf16", 1e-6, 1e24), ("fp16", 1e-2, 1e4)):
+        query, *rest = case_of(form, torch.float32, 1.0, 1.0, 0, "first")
+        query = query * low
+        head = heads - 1 if large < 0 else large
+        at = torch.arange(seqs) * rows + (rows - 1 if large else 0)
+        query[at, head] *= high / low
+        assert torch.isfinite(query.to(TYPES[dtype])).all()
+        check(ops, cuda, form, (query.to(TYPES[dtype]), *rest), scale=d**-0.5 / low)

@@ -25,7 +25,7 @@
 // with zero_j near the code that would stand for 0 (any number is right), and w_j zero_j taken off with the rounded w_j, in a
 // matrix instruction of its own: a rounding then costs about its share of the value, and nothing that the sum of p_j or the
 // second sum take depends on it, however small w_j is.  bf16 results are rounded coarser than that.  2 x 2048 queries of 64
-// heads of 128 take 755 us so in fp16, some 40 less with 7.5 for every zero_j (and 1.4 times the error), 700 in bf16.
+// heads of 128 take 758 us so in fp16, some 40 less with 7.5 for every zero_j (and 1.4 times the error), 706 in bf16.
 #include "kv4_cache.h"
 
 namespace {
@@ -125,7 +125,7 @@ struct Wave {
   int least_low;         // of all columns of the wave
   float shift[NC];       // p = 2^(score + shift)
   float sum[NC], flat[NC];
-  float unit_score;      // what makes a score (in powers of two) of a product
+  float unit_score[NC];  // what makes a score (in powers of two) of a product
   float* kept;                        // in LDS: [16 NC][D + 4], what was set aside of the sums of p v,
   float kept_sum[NC], kept_shift[NC];  // of p, and the shift that both go with
   bool keeps;
@@ -160,7 +160,7 @@ struct Wave {
   __device__ __forceinline__ void begin(const Sequence& s, int kv, int col0, int cols) {
     last_page = max(0, page_of((s.length - 1) >> 4));
     least_low = a.window > 0 ? max(0, s.before + col0 / a.group + 1 - a.window) : 0;
-    float x[NC][kSteps][8], big = 0.f, reach = 0.f;
+    float x[NC][kSteps][8], big[NC], reach = 0.f;
     const float sign = a.scale < 0.f ? -1.f : 1.f;
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
@@ -186,17 +186,15 @@ struct Wave {
       }
       qs[n] = over_groups_sum(total);
       reach = fmaxf(reach, over_groups_sum(size));
-      big = fmaxf(big, most < __builtin_inff() ? most : 0.f);  // (an infinite query is its own column's affair)
+      big[n] = over_groups_max(most < __builtin_inff() ? most : 0.f);
     }
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) big = fmaxf(big, __shfl_xor(big, m));
     far = __any(!(reach * fabsf(a.scale) * 0x1p17f < kFar));
-    // All columns by one power of two, the largest element into [2^13, 2^14): a sixteenth of it, and of what is far below
-    // it, is still a normal fp16 number, and what is not is 2^-38 of the largest score.
-    const int e = 14 - __builtin_amdgcn_frexp_expf(big);
-    unit_score = __builtin_ldexpf(fabsf(a.scale), 24 - e);
+    // Each column by a power of two of its own, its largest element into [2^13, 2^14): a sixteenth of it, and of what is far
+    // below it, is still a normal fp16 number, and what is not is 2^-38 of the column's largest score.
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
+      const int e = 14 - __builtin_amdgcn_frexp_expf(big[n]);
+      unit_score[n] = __builtin_ldexpf(fabsf(a.scale), 24 - e);
 #pragma unroll
       for (int j = 0; j < kSteps; ++j) {
 #pragma unroll
@@ -205,7 +203,7 @@ struct Wave {
           q[n][j][i] = (f16)__builtin_ldexpf(x[n][j][el], (i >> 1) & 1 ? e - 4 : e);
         }
       }
-      qs[n] = __builtin_ldexpf(qs[n], e - 24) * unit_score;
+      qs[n] = __builtin_ldexpf(qs[n], e - 24) * unit_score[n];
       shift[n] = -kNone;
       sum[n] = flat[n] = 0.f;
 #pragma unroll
@@ -278,13 +276,16 @@ struct Wave {
     return key >= low[n] && key < lim[n];
   }
 
-  // Scores of 32 keys to weights, the B operand of the second product.  ks: the keys' scales in the unit of the scores;
-  // level: what the values' codes of zero stand for (kCentred); limit: no p above 2^limit makes a p vscale of this lane
-  // pass 2^kMostWeight.
+  // Scores of 32 keys to weights, the B operand of the second product.  level: what the values' codes of zero stand for
+  // (kCentred); limit: no p above 2^limit makes a p vscale of this lane pass 2^kMostWeight.
   template <bool MASK>
-  __device__ __forceinline__ void weigh(const f32x4 (&s)[2], int n, int from, const float (&ks)[8], const float (&level)[8],
-                                        float limit, f16x8& p) {
-    float t[8];
+  __device__ __forceinline__ void weigh(const f32x4 (&s)[2], int n, int from, const float (&level)[8], float limit, f16x8& p) {
+    float t[8], ks[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      ks[i] = (float)as_pair(kp[i / 4][i % 4]).x * unit_score[n];
+      if (MASK && !known_now[i / 4]) ks[i] = __builtin_nanf("");  // of a block that the cache does not have
+    }
     const auto score = [&](int i, float more) {
       return __builtin_fmaf(ks[i], s[i / 4][i % 4], __builtin_fmaf((float)as_pair(kp[i / 4][i % 4]).y, qs[n], more));
     };
@@ -377,12 +378,6 @@ struct Wave {
 #pragma unroll
     for (int i = 1; i < 8; ++i) big = __builtin_elementwise_max(big, as_pair(vp[i / 4][i % 4]));
     const float limit = kMostWeight - (float)__builtin_amdgcn_frexp_expf(fmaxf((float)big.x, kLeastScale));
-    float ks[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      ks[i] = (float)as_pair(kp[i / 4][i % 4]).x * unit_score;
-      if (MASK && !known_now[i / 4]) ks[i] = __builtin_nanf("");  // of a block that the cache does not have
-    }
     f16x8 p[NC], zero;  // (zero: negative)
     float level[8];
     if (kCentred) {
@@ -396,7 +391,7 @@ struct Wave {
       }
     }
 #pragma unroll
-    for (int n = 0; n < NC; ++n) weigh<MASK>(s[n], n, from, ks, level, limit, p[n]);
+    for (int n = 0; n < NC; ++n) weigh<MASK>(s[n], n, from, level, limit, p[n]);
     load_params();
     // pairs of neighbouring keys side by side: 16 bits (4 elements) of each in one word
 #pragma unroll
