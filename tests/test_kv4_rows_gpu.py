@@ -321,3 +321,13 @@ def test_many_short_sequences_of_several_rows(ops, cuda, seqs, rows, heads, kv, 
     check_attend(ops, cuda, attend_case(lens, counts, heads, kv, 64, 16, TYPES[dtype], seqs), window=window)
     counts[1], lens[1] = 3 * rows, 4 * rows
     check_attend(ops, cuda, attend_case(lens, counts, heads, kv, 64, 16, TYPES[dtype], seqs), window=window)
+
+
+@pytest.mark.parametrize("lens,counts,heads,kv", [([700], [600], 128, 1), ([900, 40], [3, 2], 64, 1), ([2600], [5], 8, 2)])
+def test_more_rows_promised_than_there_are(ops, cuda, lens, counts, heads, kv):
+    """An upper bound that is far too high, beyond 32 bits of columns too, changes no bit."""
+    query, cache, tables, lens_, start = [x.to(cuda) for x in attend_case(lens, counts, heads, kv, 64, 16, torch.float16, 113)]
+    run = lambda rows: ops.paged_attention_kv4(query, cache, tables, lens_, 0.125, max(lens), query_start=start, max_query_len=rows)  # noqa: E731
+    want = run(sum(counts))
+    for rows in (32768, 10**6, (1 << 30) + 1, 0x7fffffff):
+        assert torch.equal(run(rows), want)

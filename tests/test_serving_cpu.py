@@ -282,3 +282,15 @@ def test_slots_of_positions():
     got = slots_of(tables, torch.tensor([0, 31, 32, 15, 16, 10**9]), 16, torch.tensor([0, 0, 0, 1, 1, 2]))
     assert got.tolist() == [80, 47, -1, 127, -1, -1]
     assert slots_of(tables[:, :0], torch.tensor([0, 1, -1]), 16).tolist() == [-1, -1, -1]
+
+
+def test_a_promise_of_more_rows_than_there_are(lib):
+    """max_query_len is an upper bound: one far above the rows of the batch asks for what the rows themselves do."""
+    for tokens, seqs, heads, kv, most in ((4, 2, 128, 1, 65536), (600, 1, 128, 1, 65536), (5, 2, 64, 1, 100000), (7, 3, 65535, 1, 3000)):
+        want = lib.serving_attend_kv4_workspace_bytes(tokens, seqs, heads, kv, 128, tokens, most, 0)
+        for rows in (tokens + 1, 32768, 1 << 30, (1 << 30) + 1, 0x7fffffff):
+            assert lib.serving_attend_kv4_workspace_bytes(tokens, seqs, heads, kv, 128, rows, most, 0) == want, (tokens, rows)
+            if want:  # (refused for that alone)
+                assert attend(lib, tokens=tokens, seqs=seqs, heads=heads, kv=kv, most=most, most_q=rows, ws=None) == -9
+    assert lib.serving_attend_kv4_workspace_bytes(0x7fffffff, 0x7fffffff, 65535, 1, 128, 0x7fffffff, 1 << 27, 0) == 0
+    assert attend(lib, tokens=0x7fffffff, seqs=0x7fffffff, heads=65535, kv=1, most_q=0x7fffffff, most=1 << 27) == -8

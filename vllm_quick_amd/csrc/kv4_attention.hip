@@ -911,11 +911,19 @@ bool sizes_ok(int tokens, int seqs, int heads, int kv_heads, int max_query_len, 
          max_query_len > 0 && max_seq_len > 0 && max_seq_len <= (1 << 27) && window >= 0;
 }
 
+// What a plan can count in: rows and heads, sequences and kv heads.
+bool countable(int tokens, int seqs, int heads, int kv_heads) {
+  return (long long)seqs * kv_heads <= 0x7fffffLL && (long long)tokens * heads <= 0x7fffffffLL;
+}
+
 }  // namespace
 
 extern "C" size_t serving_attend_kv4_workspace_bytes(int tokens, int seqs, int heads, int kv_heads, int head_size,
                                                      int max_query_len, int max_seq_len, int window) {
-  if (!sizes_ok(tokens, seqs, heads, kv_heads, max_query_len, max_seq_len, window) || !head_size_ok(head_size)) return 0;
+  if (!sizes_ok(tokens, seqs, heads, kv_heads, max_query_len, max_seq_len, window) || !head_size_ok(head_size) ||
+      !countable(tokens, seqs, heads, kv_heads))
+    return 0;
+  max_query_len = max_query_len < tokens ? max_query_len : tokens;  // (no sequence has more rows than there are)
   const Plan p = plan(tokens, seqs, heads, kv_heads, max_query_len, max_seq_len, window, head_size);
   return workspace_of(p, tokens, heads, head_size);
 }
@@ -935,9 +943,11 @@ extern "C" int serving_attend_kv4(const void* query, long long q_token, long lon
     return SERVING_E_SHAPE;
   if ((long long)table_width * block_size > (1LL << 27)) return SERVING_E_TOO_LARGE;
   if (!aligned16(query) || !aligned16(cache) || !aligned16(out) || q_token % 8 || q_head % 8) return SERVING_E_ALIGN;
+  if (!countable(tokens, seqs, heads, kv_heads)) return SERVING_E_TOO_LARGE;
+  max_query_len = max_query_len < tokens ? max_query_len : tokens;
   const Plan p = plan(tokens, seqs, heads, kv_heads, max_query_len, max_seq_len, window, head_size);
-  if ((long long)seqs * kv_heads > 0x7fffffLL || (p.prompt && seqs > 65535) || p.tiles > (p.prompt ? 4 : 1) * 65535LL ||
-      (!p.prompt && p.units * kv_heads * p.waves * 64 > 0xffffffffLL) || (long long)tokens * heads > 0x7fffffffLL)
+  if ((p.prompt && seqs > 65535) || (!p.search && p.tiles > (p.prompt ? 4 : 1) * 65535LL) ||
+      (!p.prompt && p.units * kv_heads * p.waves * 64 > 0xffffffffLL))
     return SERVING_E_TOO_LARGE;
   const size_t need = workspace_of(p, tokens, heads, head_size);
   if (need && (!workspace || workspace_bytes < need)) return SERVING_E_WORKSPACE;
