@@ -331,3 +331,17 @@ def test_more_rows_promised_than_there_are(ops, cuda, lens, counts, heads, kv):
     want = run(sum(counts))
     for rows in (32768, 10**6, (1 << 30) + 1, 0x7fffffff):
         assert torch.equal(run(rows), want)
+
+
+def test_more_sequences_than_a_grid_has_in_one_direction(ops, cuda):
+    """70 000 sequences of three drafted tokens and 24 heads, which are columns enough for waves of their own."""
+    seqs, rows, heads, d, p = 70000, 3, 24, 64, 16
+    few = attend_case([9, 3, 16, 5], [rows] * 4, heads, 1, d, p, torch.float16, 127)
+    query, cache, tables, lens, _ = [x.to(cuda) for x in few]
+    again = lambda t: t.repeat(seqs // 4, *[1] * (t.dim() - 1))  # noqa: E731
+    start = torch.arange(seqs + 1, dtype=torch.int32, device=cuda) * rows
+    got = ops.paged_attention_kv4(again(query), cache, again(tables), again(lens), 0.125, 16, query_start=start, max_query_len=rows)
+    want, tol = orc.attend(*few, 0.125, 0, True)
+    for at in (0, 65532 * rows, (seqs - 4) * rows):
+        assert ((got[at:at + 4 * rows].cpu().double() - want).abs() <= tol).all()
+    assert torch.equal(got.view(seqs // 4, -1), got[:4 * rows].view(1, -1).expand(seqs // 4, -1))

@@ -815,7 +815,8 @@ Plan plan(int tokens, int seqs, int heads, int kv_heads, int max_query_len, int 
   // sequence's 512 queries of 8 x 4 heads over 8192 keys 268 and 102, one query of 128 heads over 65536 keys 2070 and 27;
   // 2048 queries beside 63 single ones, each over 4096 keys, 995 and 222.  Long sequences want a second such round
   // (2048 queries of 8 x 4 heads over 65536 keys, one round: 2970 and 2710; twice 2048 over 8192, two: 633 and 630).
-  p.prompt = cols > 64 && full * kv_heads >= (max_seq_len > 2048 ? 4096 : 2048) && 2 * full >= most_tiles;
+  // (A grid takes 65535 in the direction that its sequences, and its groups of four tiles, have to themselves.)
+  p.prompt = cols > 64 && full * kv_heads >= (max_seq_len > 2048 ? 4096 : 2048) && 2 * full >= most_tiles && seqs <= 65535;
   if (p.prompt) return p;
   long long keys = max_seq_len;
   if (window > 0 && (long long)window + max_query_len < keys) keys = window + max_query_len;
@@ -946,7 +947,7 @@ extern "C" int serving_attend_kv4(const void* query, long long q_token, long lon
   if (!countable(tokens, seqs, heads, kv_heads)) return SERVING_E_TOO_LARGE;
   max_query_len = max_query_len < tokens ? max_query_len : tokens;
   const Plan p = plan(tokens, seqs, heads, kv_heads, max_query_len, max_seq_len, window, head_size);
-  if ((p.prompt && seqs > 65535) || (!p.search && p.tiles > (p.prompt ? 4 : 1) * 65535LL) ||
+  if ((!p.search && p.tiles > (p.prompt ? 4 : 1) * 65535LL) ||
       (!p.prompt && p.units * kv_heads * p.waves * 64 > 0xffffffffLL))
     return SERVING_E_TOO_LARGE;
   const size_t need = workspace_of(p, tokens, heads, head_size);
