@@ -3,6 +3,8 @@ and the oracle's own pieces against each other."""
 import ctypes
 import os
 import re
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -294,3 +296,24 @@ def test_a_promise_of_more_rows_than_there_are(lib):
                 assert attend(lib, tokens=tokens, seqs=seqs, heads=heads, kv=kv, most=most, most_q=rows, ws=None) == -9
     assert lib.serving_attend_kv4_workspace_bytes(0x7fffffff, 0x7fffffff, 65535, 1, 128, 0x7fffffff, 1 << 27, 0) == 0
     assert attend(lib, tokens=0x7fffffff, seqs=0x7fffffff, heads=65535, kv=1, most_q=0x7fffffff, most=1 << 27) == -8
+
+
+def test_awq_operators_do_without_the_torch_extension():
+    """Where only libw4a16.so is built the AWQ operators import as they are, and the others say what is missing."""
+    code = """
+import sys
+sys.modules["vllm_quick_amd._C_native"] = None  # its import fails
+import torch
+from vllm_quick_amd import ops
+from vllm_quick_amd.layers.linear import ColumnParallelLinear
+assert callable(ops.awq_gemm) and callable(ops.awq_dequantize)
+cache = ops.kv4_cache(2, 16, 2, 64, torch.device("cpu"))
+try:
+    ops.kv4_read(cache, torch.zeros(1, dtype=torch.int64), 64, torch.float16)
+except ImportError as e:
+    assert "_C_native" in str(e)
+else:
+    raise AssertionError
+"""
+    done = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-1500:]

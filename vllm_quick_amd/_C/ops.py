@@ -21,10 +21,7 @@ from typing import Dict, Optional, Sequence, Tuple
 
 import torch
 
-from .. import _C_native
 from .._lib import check, lib
-
-_native = _C_native.ops
 
 PACK_FACTOR = 8
 
@@ -699,6 +696,18 @@ def awq_dequantize_packed(packed: PackedAWQ) -> torch.Tensor:
 # --------------------------------------------------------------------------
 # around the products of a generating step (libserving_ops.so, include/serving_ops.h)
 # --------------------------------------------------------------------------
+_native_ops = None
+
+
+def _native():
+    """The operators of the torch extension, which those of libw4a16.so do without: ImportError where it is not built."""
+    global _native_ops
+    if _native_ops is None:
+        from .. import _C_native
+        _native_ops = _C_native.ops
+    return _native_ops
+
+
 def kv4_cache(num_blocks: int, block_size: int, num_kv_heads: int, head_size: int, device: torch.device) -> torch.Tensor:
     """A zeroed paged cache of keys and values in 4 bits: uint8 [num_blocks, num_kv_heads, block_size * (head_size + 8)],
     a scale and a least value (fp16) for each head of each token; the format is in include/serving_ops.h.  head_size is
@@ -723,14 +732,14 @@ def rope_append_kv4(positions: torch.Tensor, query: torch.Tensor, key: torch.Ten
     `rotary` (a multiple of 16, 0 for none) elements of each head turn, in pairs (i, i + rotary / 2) or, `interleaved`,
     (2 i, 2 i + 1).  slot = block * block_size + place; a slot outside the cache (a padded row's -1) stores nothing; the
     others have to differ.  A position outside cos_sin makes NaN of what would turn."""
-    return _native.rope_append_kv4(positions, query, key, value, cos_sin, cache, slots, interleaved)
+    return _native().rope_append_kv4(positions, query, key, value, cos_sin, cache, slots, interleaved)
 
 
 def kv4_read(cache: torch.Tensor, slots: torch.Tensor, head_size: int,
              dtype: torch.dtype) -> Tuple[torch.Tensor, torch.Tensor]:
     """What slots (int64 [n]) of a 4-bit cache stand for: key and value [n, kv_heads, head_size] in fp16 or bf16, each
     `least + code * scale` rounded once; zeros for a slot outside the cache."""
-    return _native.kv4_read(cache, slots, head_size, dtype)
+    return _native().kv4_read(cache, slots, head_size, dtype)
 
 
 def paged_attention_kv4(query: torch.Tensor, cache: torch.Tensor, block_tables: torch.Tensor, seq_lens: torch.Tensor,
@@ -744,8 +753,8 @@ def paged_attention_kv4(query: torch.Tensor, cache: torch.Tensor, block_tables: 
     and each sees what stands up to itself; window > 0: the last `window` of that.  max_seq_len and max_query_len size
     the launch; rows past max_query_len of a sequence come back NaN.  A row that sees nothing is zero; rows of no
     sequence are left as `out` holds them.  `out` may be the query itself."""
-    return _native.paged_attention_kv4(query, cache, block_tables, seq_lens, scale, max_seq_len, query_start, max_query_len,
-                                       window, out)
+    return _native().paged_attention_kv4(query, cache, block_tables, seq_lens, scale, max_seq_len, query_start, max_query_len,
+                                         window, out)
 
 
 def token_logprobs(logits: torch.Tensor, token_ids: torch.Tensor,
@@ -754,4 +763,4 @@ def token_logprobs(logits: torch.Tensor, token_ids: torch.Tensor,
     outside the vocabulary) and the entropy, fp32 [R], and the top_n (0 .. 64) most likely tokens, int64 [R, top_n], the
     lowest index first among equals, with their log probabilities, fp32 [R, top_n].  A logit of -inf is no token; a row
     without any, or with a NaN or +inf, has NaN for all its probabilities."""
-    return _native.token_logprobs(logits, token_ids, top_n)
+    return _native().token_logprobs(logits, token_ids, top_n)
