@@ -345,3 +345,28 @@ def test_more_sequences_than_a_grid_has_in_one_direction(ops, cuda):
     for at in (0, 65532 * rows, (seqs - 4) * rows):
         assert ((got[at:at + 4 * rows].cpu().double() - want).abs() <= tol).all()
     assert torch.equal(got.view(seqs // 4, -1), got[:4 * rows].view(1, -1).expand(seqs // 4, -1))
+
+
+def test_tangents_are_refused(ops, cuda):
+    """Forward-mode differentiation: no result that silently lacks its tangent."""
+    import torch.autograd.forward_ad as fwad
+    query, cache, tables, lens, start = [x.to(cuda) for x in attend_case([30, 4], [1, 1], 4, 2, 64, 16, torch.float16, 83)]
+    slots = torch.tensor([0, 40], device=cuda)
+    kv = torch.zeros(2, 2, 64, dtype=torch.float16, device=cuda)
+    cs = torch.zeros(41, 64, device=cuda)
+    calls = [(query, lambda x: ops.paged_attention_kv4(x, cache, tables, lens, 0.1, 30)),
+             (query, lambda x: ops.paged_attention_kv4(query, cache, tables, lens, 0.1, 30, out=x)),
+             (query, lambda x: ops.rope_append_kv4(slots, x, kv, kv, cs, cache, slots)),
+             (kv, lambda x: ops.rope_append_kv4(slots, query, x, kv, cs, cache, slots)),
+             (kv, lambda x: ops.rope_append_kv4(slots, query, kv, x, cs, cache, slots)),
+             (cs, lambda x: ops.rope_append_kv4(slots, query, kv, kv, x, cache, slots)),
+             (query.view(2, -1), lambda x: ops.token_logprobs(x, slots, 1))]
+    for of, call in calls:
+        with fwad.dual_level():
+            dual = fwad.make_dual(of.clone(), torch.ones_like(of))
+            with pytest.raises(RuntimeError, match="tangent"):
+                call(dual)
+            with torch.no_grad(), pytest.raises(RuntimeError, match="tangent"):
+                call(dual)
+            call(fwad.unpack_dual(dual).primal)
+        call(of.clone())

@@ -7,6 +7,7 @@
 #include <ATen/hip/HIPContext.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <c10/core/AutogradState.h>
 #include <torch/extension.h>
 
 #include <optional>
@@ -71,6 +72,8 @@ void on_gpu(const Tensor& t, const Tensor& like, const char* what, const char* n
 void no_gradient(const Tensor& t, const char* what, const char* name) {
   TORCH_CHECK(!(at::GradMode::is_enabled() && t.requires_grad()), what, ": ", name,
               " requires a gradient, which this operator does not give: call it under torch.no_grad() or on a detached tensor");
+  TORCH_CHECK(!(c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined()), what, ": ", name,
+              " carries a tangent of forward-mode differentiation, which this operator does not pass on");
 }
 
 // What a call writes into counts as changed in place for whoever saved it for a backward pass.
