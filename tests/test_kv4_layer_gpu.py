@@ -131,3 +131,37 @@ def test_captured_harness_step_chooses_what_the_eager_one_does(cuda):
                 assert torch.equal(a, b)
             assert torch.equal(want[0], want[2][:, 0]) and (want[1][:, :-1] >= want[1][:, 1:]).all()
             tokens.copy_(want[0])
+
+
+@pytest.mark.parametrize("window,interleaved", [(0, False), (25, True)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_layer_against_the_oracle_with_nothing_to_spare(cuda, dtype, window, interleaved):
+    """Prompts and tokens through the layer, the oracle given the queries as the operator rotates them (which has tests of
+    its own), so that attention's counted roundings are all that is allowed."""
+    from vllm_quick_amd import ops
+    from vllm_quick_amd.layers.kv4_attention import KV4Attention, KV4Metadata, rope_table, slots_of
+    heads, kv, d, p = 6, 2, 64, 16
+    attn = KV4Attention(heads, d, kv, window=window, interleaved=interleaved)
+    cache = attn.make_cache(9, p, cuda)
+    cos_sin = rope_table(64, d, device=cuda)
+    tables = torch.tensor([[3, 7, 1], [8, 0, 5]], dtype=torch.int32, device=cuda)
+    g = torch.Generator().manual_seed(4)
+    lens = [0, 0]
+    for counts in ([20, 33], [1, 1], [3, 0], [1, 1], [20, 9]):
+        t = sum(counts)
+        qkv = torch.randn(t, (heads + 2 * kv) * d, generator=g).to(dtype).to(cuda)
+        q, k, v = qkv.split([heads * d, kv * d, kv * d], 1)
+        pos = torch.cat([torch.arange(n, n + m) for n, m in zip(lens, counts)]).to(cuda)
+        seq = torch.repeat_interleave(torch.arange(2), torch.tensor(counts)).to(cuda)
+        lens = [n + m for n, m in zip(lens, counts)]
+        start = torch.tensor([0, counts[0], t], dtype=torch.int32, device=cuda)
+        seq_lens = torch.tensor(lens, dtype=torch.int32, device=cuda)
+        single = counts == [1, 1]
+        slots = slots_of(tables, pos, p, seq)
+        meta = KV4Metadata(pos, slots, tables, seq_lens, max(lens), None if single else start, 1 if single else max(counts))
+        beside = cache.clone()
+        turned = ops.rope_append_kv4(pos, q.view(t, heads, d), k.view(t, kv, d), v.view(t, kv, d), cos_sin, beside, slots, interleaved)
+        out = attn(q, k, v, cache, cos_sin, meta).view(t, heads, d)
+        assert torch.equal(cache, beside)
+        want, tol = orc.attend(turned.cpu(), cache.cpu(), tables.cpu(), seq_lens.cpu(), start.cpu(), d**-0.5, window, dtype == torch.float16)
+        assert ((out.cpu().double() - want).abs() <= tol).all()
