@@ -92,7 +92,13 @@ int serving_read_kv4(const void* cache, const int64_t* slots, void* key, void* v
  * query_start NULL: one row for each sequence (tokens = seqs).  heads is a multiple of kv_heads; query head h reads
  * kv head h / (heads / kv_heads).  A row that sees no key gives zeros; rows of no sequence are left as they were; rows
  * past the first max_query_len of a sequence are NaN; keys in a block outside the cache are NaN.  max_query_len and
- * max_seq_len size the launch only: a sequence longer than max_seq_len is still read whole.
+ * max_seq_len size the launch only: a sequence longer than max_seq_len is still read whole, and a max_query_len above
+ * `tokens` counts as `tokens`.
+ * Arithmetic: products of fp16 numbers summed in fp32; a weight, p times the scale of its token's values, is rounded to
+ * fp16 once, against the largest of the row's, whose rounding a result of fp16 has times the value itself and one of
+ * bf16 times up to 15 codes; results are rounded once.  A row's result does not depend on keys that it does not see, nor
+ * on how large other rows are.  Scores have to be finite in fp32.  Queries whose absolute values add up to more than
+ * 2^8 / |scale * log2(e)| make their column tile run the slower steps that masks take (1.7 times as long for a prompt).
  * workspace: serving_attend_kv4_workspace_bytes() of the same arguments (0: none needed), used by one launch at a
  * time, nothing is kept in it.
  */
@@ -112,6 +118,7 @@ int serving_attend_kv4(const void* query, long long q_token, long long q_head, c
  *   top_ids[r], top_logprobs[r] [rows, top]: the `top` (0 .. 64) most likely tokens, the most likely first, among
  *                 equals the lowest index first (both zeros are equal, a NaN ranks above all numbers).
  * A row that is -inf throughout, or holds a NaN or +inf, has NaN for all its probabilities, as the formulas give.
+ * Arithmetic: exponentials and their sums in fp32, the logarithm and what follows in 64 bits, results rounded once.
  * logprob, entropy, top_logprobs fp32; token_ids and top_ids int64.
  */
 size_t serving_token_logprobs_workspace_bytes(int rows, int vocab, int top, int type);
