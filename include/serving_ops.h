@@ -97,9 +97,9 @@ int serving_read_kv4(const void* cache, const int64_t* slots, void* key, void* v
  * Arithmetic: products of fp16 numbers summed in fp32; a weight, p times the scale of its token's values, is rounded to
  * fp16 once, against the largest of the row's, whose rounding a result of fp16 has times the value itself and one of
  * bf16 times up to 15 codes; results are rounded once.  A row's result does not depend on keys that it does not see, nor,
- * but for roundings of fp32, on how large other rows are.  Scores have to be finite in fp32.  Queries whose absolute
- * values add up to more than 2^8 / |scale * log2(e)| make their column tile run the slower steps that masks take (1.7
- * times as long for a prompt).
+ * but for roundings of fp32, on how large other rows are.  Scores have to be finite in fp32, and below 2^115 what the
+ * scale, a query's largest element and a key's multiply to; rows with scores beyond 2^25 make their column tile take the
+ * slower steps of masks (1.7 times as long for a prompt).
  * workspace: serving_attend_kv4_workspace_bytes() of the same arguments (0: none needed), used by one launch at a
  * time, nothing is kept in it.
  */

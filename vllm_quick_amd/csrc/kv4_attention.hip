@@ -25,7 +25,7 @@
 // with zero_j near the code that would stand for 0 (any number is right), and w_j zero_j taken off with the rounded w_j, in a
 // matrix instruction of its own: a rounding then costs about its share of the value, and nothing that the sum of p_j or the
 // second sum take depends on it, however small w_j is.  bf16 results are rounded coarser than that.  2 x 2048 queries of 64
-// heads of 128 take 758 us so in fp16, some 40 less with 7.5 for every zero_j (and 1.4 times the error), 706 in bf16.
+// heads of 128 take 770 us so in fp16, some 40 less with 7.5 for every zero_j (and 1.4 times the error), 712 in bf16.
 #include "kv4_cache.h"
 
 namespace {
@@ -39,9 +39,8 @@ constexpr float kWeightLog = 7.f;      // what a column is held against is set s
 constexpr float kMostWeight = 15.f;    // and again when one may pass 2^15, which fp16 holds
 constexpr float kLeastScale = 0x1p-24f;  // of a token whose values are all alike, for that purpose: fp16's least number
 
-// Scores beyond kFar have digits of 4 and more: what fp16 holds of a weight would be their roundings'.  A query whose
-// absolute values, times the scale, stay below 2^-17 of it in sum has none (a key is below 2^17); 2 x 2048 queries that
-// may have some, 20 times unit normal numbers, take 2170 us over 8192 keys instead of 1240.
+// Scores beyond kFar have digits of 4 and more: a wave that is held against one rounds scores by themselves from then on,
+// in steps that take 1.7 times as long.
 constexpr float kFar = 0x1p25f;
 
 struct AttendArgs {
@@ -87,8 +86,12 @@ __device__ __forceinline__ float over_groups_sum(float v) {
   return v + __shfl_xor(v, 32);
 }
 
-// Keeps a branch that is rarely taken a branch.
-__device__ __forceinline__ void stay() { asm volatile(""); }
+// Keeps what is worked out of x in a branch that is rarely taken out of the registers before it.
+template <typename V>
+__device__ __forceinline__ V here(V x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
 
 // One sequence as a wave sees it.
 struct Sequence {
@@ -130,7 +133,7 @@ struct Wave {
   float* kept;                        // in LDS: [16 NC][D + 4], what was set aside of the sums of p v,
   float kept_sum[NC], kept_shift[NC];  // of p, and the shift that both go with
   bool keeps;
-  bool far;  // some column's scores may pass kFar: all steps are taken as those with masks then, which see to it
+  bool far;  // some column is held against a score beyond kFar: steps are taken as those with masks, which see to that
   f32x4 o[NC][kRows], off[NC];  // sums of w code and, in each element, of w (- zero) (kCentred)
   const uint8_t* head_base;  // of this kv head in block 0
   scalar_ints table;
@@ -146,7 +149,7 @@ struct Wave {
   // some block of the table, or block 0, holds, and nobody looks at it.
   __device__ __forceinline__ void first_loads(int b, int kv, int first, float* lds) {
     kept = lds;
-    keeps = false;
+    keeps = far = false;
     head_base = a.cache + (long long)kv * Kv4<D>::block_bytes(a.block_size);
     block_bytes = Kv4<D>::block_bytes(a.block_size) * a.kv_heads;
     table = scalar(a.tables + b * a.table_stride);
@@ -161,7 +164,7 @@ struct Wave {
   __device__ __forceinline__ void begin(const Sequence& s, int kv, int col0, int cols) {
     last_page = max(0, page_of((s.length - 1) >> 4));
     least_low = a.window > 0 ? max(0, s.before + col0 / a.group + 1 - a.window) : 0;
-    float x[NC][kSteps][8], big[NC], reach = 0.f;
+    float x[NC][kSteps][8], big[NC];
     const float sign = a.scale < 0.f ? -1.f : 1.f;
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
@@ -172,7 +175,7 @@ struct Wave {
       low[n] = a.window > 0 ? max(0, lim[n] - a.window) : 0;
       const T* src = static_cast<const T*>(a.query) + (long long)(s.row + qi) * a.q_token + (kv * a.group + h) * a.q_head;
       typedef T vec8 __attribute__((ext_vector_type(8)));
-      float most = 0.f, total = 0.f, size = 0.f;
+      float most = 0.f, total = 0.f;
 #pragma unroll
       for (int j = 0; j < kSteps; ++j) {
         vec8 w = {};
@@ -181,15 +184,12 @@ struct Wave {
         for (int i = 0; i < 8; ++i) {
           x[n][j][i] = sign * (float)w[i];
           most = fmaxf(most, fabsf(x[n][j][i]));
-          size += fabsf(x[n][j][i]);
           total += x[n][j][i];
         }
       }
       qs[n] = over_groups_sum(total);
-      reach = fmaxf(reach, over_groups_sum(size));
       big[n] = over_groups_max(most < __builtin_inff() ? most : 0.f);
     }
-    far = __any(!(reach * fabsf(a.scale) * 0x1p17f < kFar));
     // Each column by a power of two of its own, its largest element into [2^13, 2^14): a sixteenth of it, and of what is far
     // below it, is still a normal fp16 number, and what is not is 2^-38 of the column's largest score.
 #pragma unroll
@@ -299,25 +299,55 @@ struct Wave {
 #pragma unroll
     for (int i = 1; i < 8; ++i) most = fmaxf(most, t[i]);
     if (__any(most > limit)) {
-      stay();
-      float passed = kNone, top = kNone, peak = kNone;  // of score + log2 vscale, or a little above it; of scores
+      const auto log_scale = [&](int i) {
+        return (float)__builtin_amdgcn_frexp_expf(fmaxf((float)as_pair(here(vp[i / 4][i % 4])).x, kLeastScale));
+      };
+      const auto heaviest = [&] {  // log2 of the largest p vscale, or a little above it
+        float x = kNone;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x = fmaxf(x, t[i] + log_scale(i));
+        return over_groups_max(x);
+      };
+      // (a column moves for its own keys only, whatever the wave's others do)
+      float passed = kNone, top = kNone;  // of score + log2 vscale, or a little above it
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        uint32_t par = vp[i / 4][i % 4];
-        asm volatile("" : "+v"(par));  // (worked out here, not kept in registers for here)
-        const float log_scale = (float)__builtin_amdgcn_frexp_expf(fmaxf((float)as_pair(par).x, kLeastScale));
-        passed = fmaxf(passed, t[i] + log_scale);
-        if (MASK && !sees(n, from, i)) continue;
-        const float x = MASK ? score(i, 0.f) : 0.f;
-        peak = fmaxf(peak, x);
-        top = fmaxf(top, MASK ? x + log_scale : score(i, log_scale));
+        const float more = log_scale(i);
+        passed = fmaxf(passed, t[i] + more);
+        if (!MASK) top = fmaxf(top, score(i, more));
       }
-      // (a column moves for its own keys only, whatever the wave's others do)
       const bool moves = over_groups_max(passed) > kMostWeight;
-      float next = moves ? kWeightLog - over_groups_max(top) : shift[n];
-      if (MASK) {
-        peak = over_groups_max(peak);
-        if (moves && fabsf(peak) >= kFar) next = -peak;
+      bool aside = moves;
+      float next = shift[n];
+      if (!MASK) {
+        top = over_groups_max(top);
+        next = moves ? fminf(kWeightLog - top, next) : next;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) t[i] = score(i, next);  // (rounded as outside, which other columns may have called for)
+        aside = moves && (fabsf(top) >= kFar || fabsf(qs[n]) * 0x1p16f >= kFar);  // (a key's least value is below 2^16)
+      }
+      // A far score, or what a far score's parts have put aside of where it was to come: a score is rounded by itself then, so
+      // that its difference to what it is held against is that of two scores.
+      if (MASK || __any(aside)) {
+        if (!MASK) aside = aside && !(fabsf(heaviest() - kWeightLog) <= 4.f && fabsf(next) < kFar);
+        float peak = kNone;
+        top = kNone;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (MASK && !sees(n, from, i)) continue;
+          const float x = score(i, here(0.f));
+          peak = fmaxf(peak, x);
+          top = fmaxf(top, x + log_scale(i));
+        }
+        peak = over_groups_max(peak), top = over_groups_max(top);
+        const bool beyond = fabsf(peak) >= kFar;
+        next = aside ? fminf(beyond ? -peak : kWeightLog - top, shift[n]) : next;
+        far |= __any(aside && (!MASK || beyond));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (MASK || aside) t[i] = score(i, here(0.f)) + next;
+          if (MASK) t[i] = sees(n, from, i) ? t[i] : kNone;
+        }
       }
       const float f = exp2_(next - shift[n]);
       shift[n] = next;
@@ -326,11 +356,6 @@ struct Wave {
 #pragma unroll
       for (int m = 0; m < kRows; ++m) o[n][m] *= f;
       off[n] *= f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {  // (rounded as outside of this branch, which other columns may have called for)
-        t[i] = MASK ? score(i, 0.f) + next : score(i, next);
-        if (MASK) t[i] = sees(n, from, i) ? t[i] : kNone;
-      }
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -738,7 +763,7 @@ __device__ __forceinline__ int by_length(const AttendArgs& a, int rank) {
 // Many queries a sequence: each wave has columns of its own and runs over all the keys that they see; the four waves of
 // a workgroup hold neighbouring columns, so that they read the same keys at about the same time.  Vector instructions
 // bound it (261 and 16 exponentials for 32 matrix instructions in bf16, 293 and 16 for 34 in fp16): 2 x 2048 queries of 64
-// heads of 128 over 2500 and 8192 keys take 707 us (758 in fp16), 0.78 PFLOP/s.  Converting each code once a workgroup,
+// heads of 128 over 2500 and 8192 keys take 712 us (770 in fp16), 0.77 PFLOP/s.  Converting each code once a workgroup,
 // through LDS, takes a quarter of them away and costs more in waits than that (740 us with two barriers a step).
 template <typename T, int D, int NC>
 __global__ void __launch_bounds__(256, D == 64 ? 3 : 2) attend_prompt_kernel(AttendArgs a) {
